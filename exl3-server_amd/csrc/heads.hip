@@ -1,0 +1,186 @@
+// The norm of every query and key head with the position rotation behind it (gfx950).
+//
+//   y = x * r * w,  r = 1 / sqrt(mean(x^2) + eps) (RMS) or 1 / sqrt(sum(x^2) + eps) (L2)
+//   of the first R values of a head, pairs (a, b) = (y[i], y[i + R/2]) or (y[2i], y[2i + 1]):
+//   (a cos - b sin, b cos + a sin), angle = position * inv_freq[i]
+//
+// Statistics, products and the rotation are f32; the result is rounded once. An angle is
+// taken in f64 and reduced to turns there: position * inv_freq has up to 55 bits, and at
+// position 10^6 an f32 product is off by 0.06 of a radian.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <string>
+
+#include "elem.hpp"
+#include "exl3_device.hpp"
+#include "exl3_internal.hpp"
+#include "exl3_moe.h"
+
+using namespace exl3d;
+using namespace exl3e;
+
+namespace {
+
+constexpr int kMaxHeadDim = 1024;
+
+struct HeadSide {
+  const void *x, *w;
+  void *y;
+  int32_t heads;
+  int64_t x_token, x_head, y_token, y_head;
+};
+
+struct HeadArgs {
+  HeadSide s[2];
+  int64_t tokens;
+  int32_t d, R, interleaved, l2;
+  float eps;
+  const int32_t *positions;
+  const float *inv_freq;
+};
+
+// cos and sin of position * inv_freq.
+__device__ __forceinline__ float2 turn(int32_t pos, float inv_freq) {
+  const double t = (double)pos * (double)inv_freq * 0.15915494309189533577;  // in turns
+  float s, c;
+  sincospif((float)(2.0 * (t - rint(t))), &s, &c);
+  return make_float2(c, s);
+}
+
+__device__ __forceinline__ float scale_of(const HeadArgs &a, float sq) {
+  return 1.0f / sqrtf((a.l2 ? sq : sq / (float)a.d) + a.eps);
+}
+
+// Any head size up to 1024, any strides: a wave per head, values one by one, the normed head
+// in LDS for the rotation's partners.
+template <typename E>
+__global__ __launch_bounds__(64) void k_head_norm_any(HeadArgs a) {
+  __shared__ float y[kMaxHeadDim];
+  const int lane = threadIdx.x;
+  const int64_t tok = blockIdx.x;
+  const int h = blockIdx.y;
+  const bool second = h >= a.s[0].heads;
+  const HeadSide &s = a.s[second ? 1 : 0];
+  const int hh = second ? h - a.s[0].heads : h;
+  const E *x = reinterpret_cast<const E *>(s.x) + tok * s.x_token + hh * s.x_head;
+  const E *w = reinterpret_cast<const E *>(s.w);
+  E *out = reinterpret_cast<E *>(s.y) + tok * s.y_token + hh * s.y_head;
+  float sq = 0.0f;
+  for (int i = lane; i < a.d; i += 64) {
+    const float v = to_f32(x[i]);
+    y[i] = v;
+    sq = fmaf(v, v, sq);
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) sq += __shfl_xor(sq, o);
+  const float r = scale_of(a, sq);
+  for (int i = lane; i < a.d; i += 64) y[i] = y[i] * r * (w ? to_f32(w[i]) : 1.0f);
+  __syncthreads();
+  const int half = a.R / 2;
+  for (int i = lane; i < half; i += 64) {
+    const float2 cs = turn(a.positions[tok], a.inv_freq[i]);
+    const int p = a.interleaved ? 2 * i : i, q = a.interleaved ? 2 * i + 1 : i + half;
+    const float u = y[p], v = y[q];
+    out[p] = from_f32<E>(u * cs.x - v * cs.y);
+    out[q] = from_f32<E>(v * cs.x + u * cs.y);
+  }
+  for (int i = a.R + lane; i < a.d; i += 64) out[i] = from_f32<E>(y[i]);
+}
+
+// Byte distance from the first to past the last value of a side's rows.
+size_t span_bytes(const HeadSide &s, bool out, int64_t T, int d) {
+  const int64_t t = out ? s.y_token : s.x_token, h = out ? s.y_head : s.x_head;
+  return (size_t)((T - 1) * t + (s.heads - 1) * h + d) * 2;
+}
+
+// Whether two sides' rows share a value: exactly where both are token-major with one token
+// stride (parts of one packed row), else where their spans meet.
+bool rows_meet(const void *pa, int64_t ta, int64_t ha, int na, const void *pb, int64_t tb, int64_t hb, int nb,
+               int64_t T, int d) {
+  const int64_t wa = (na - 1) * ha + d, wb = (nb - 1) * hb + d;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(pa), b = reinterpret_cast<uintptr_t>(pb);
+  if (ta != tb || ta < wa || ta < wb || T == 1)
+    return spans_meet(a, (size_t)((T - 1) * ta + wa) * 2, b, (size_t)((T - 1) * tb + wb) * 2);
+  const int64_t delta = (int64_t)(b - a), s = 2 * ta;
+  int64_t q = delta / s, r = delta % s;
+  if (r < 0) {
+    r += s;
+    --q;
+  }
+  // b's row t begins r bytes behind a's row t + q, and s - r bytes before a's row t + q + 1
+  return (r < 2 * wa && std::llabs(q) < T) || (s - r < 2 * wb && std::llabs(q + 1) < T);
+}
+
+}  // namespace
+
+using namespace exl3h;
+
+extern "C" exl3_status exl3_head_norm(const exl3_head_norm_config *cfg, const exl3_head_rows *q, const exl3_head_rows *k,
+                                      int64_t tokens, const int32_t *positions, const float *inv_freq,
+                                      exl3_stream_t stream) {
+  if (!cfg || !q) return fail(EXL3_ERR_INVALID, "exl3_head_norm: null argument");
+  if (cfg->dtype != EXL3_ST_F16 && cfg->dtype != EXL3_ST_BF16)
+    return fail(EXL3_ERR_UNSUPPORTED, "exl3_head_norm: dtype must be f16 or bf16");
+  if (cfg->mode != EXL3_NORM_RMS && cfg->mode != EXL3_NORM_L2)
+    return fail(EXL3_ERR_INVALID, "exl3_head_norm: unknown mode");
+  const int d = cfg->head_dim;
+  if (d < 1 || d > kMaxHeadDim) return fail(EXL3_ERR_UNSUPPORTED, "exl3_head_norm: head_dim must be 1..1024");
+  if (cfg->rotate_dims < 0 || cfg->rotate_dims > d || cfg->rotate_dims % 2)
+    return fail(EXL3_ERR_INVALID, "exl3_head_norm: rotate_dims must be even and at most head_dim");
+  if (!(cfg->eps >= 0.0f)) return fail(EXL3_ERR_INVALID, "exl3_head_norm: eps must not be negative");
+  if (tokens < 0 || tokens > ((int64_t)1 << 31) - 1) return fail(EXL3_ERR_INVALID, "exl3_head_norm: bad token count");
+  const exl3_head_rows *sides[2] = {q, k};
+  HeadArgs a = {};
+  int heads = 0;
+  for (int i = 0; i < (k ? 2 : 1); ++i) {
+    const exl3_head_rows &s = *sides[i];
+    // head counts of a launch's second dimension; strides that 2^48 elements bound cannot overflow
+    if (s.heads < 1 || s.heads > 32767) return fail(EXL3_ERR_INVALID, "exl3_head_norm: heads must be 1..32767");
+    for (int64_t v : {s.x_token, s.x_head, s.y_token, s.y_head})
+      if (v < 0 || v > ((int64_t)1 << 31) * 64) return fail(EXL3_ERR_INVALID, "exl3_head_norm: bad stride");
+    const bool token_major = (s.heads == 1 || s.y_head >= d) && (tokens <= 1 || s.y_token >= (s.heads - 1) * s.y_head + d);
+    const bool head_major = (tokens <= 1 || s.y_token >= d) && (s.heads == 1 || s.y_head >= (tokens - 1) * s.y_token + d);
+    if (!token_major && !head_major) return fail(EXL3_ERR_INVALID, "exl3_head_norm: output rows overlap each other");
+    a.s[i] = HeadSide{s.x, s.w, s.y, s.heads, s.x_token, s.x_head, s.y_token, s.y_head};
+    heads += s.heads;
+  }
+  if (tokens == 0) return EXL3_OK;
+  for (int i = 0; i < (k ? 2 : 1); ++i) {
+    const HeadSide &s = a.s[i];
+    if (!s.x || !s.y) return fail(EXL3_ERR_INVALID, "exl3_head_norm: null rows");
+    if ((reinterpret_cast<uintptr_t>(s.x) | reinterpret_cast<uintptr_t>(s.y) | reinterpret_cast<uintptr_t>(s.w)) % 2)
+      return fail(EXL3_ERR_INVALID, "exl3_head_norm: rows and weights must be 2-byte aligned");
+    for (int j = 0; j < (k ? 2 : 1); ++j) {
+      const HeadSide &o = a.s[j];
+      const bool in_place = i == j && s.x == s.y && s.x_token == s.y_token && s.x_head == s.y_head;
+      if (!in_place && rows_meet(s.y, s.y_token, s.y_head, s.heads, o.x, o.x_token, o.x_head, o.heads, tokens, d))
+        return fail(EXL3_ERR_INVALID, "exl3_head_norm: an output overlaps an input (in place: the same rows)");
+      if (o.w && spans_meet(reinterpret_cast<uintptr_t>(s.y), span_bytes(s, true, tokens, d),
+                            reinterpret_cast<uintptr_t>(o.w), (size_t)d * 2))
+        return fail(EXL3_ERR_INVALID, "exl3_head_norm: an output overlaps a weight");
+    }
+  }
+  if (k && rows_meet(a.s[0].y, a.s[0].y_token, a.s[0].y_head, a.s[0].heads, a.s[1].y, a.s[1].y_token, a.s[1].y_head,
+                     a.s[1].heads, tokens, d))
+    return fail(EXL3_ERR_INVALID, "exl3_head_norm: the outputs overlap each other");
+  if (cfg->rotate_dims) {
+    if (!positions || !inv_freq) return fail(EXL3_ERR_INVALID, "exl3_head_norm: the rotation needs positions and inv_freq");
+    if ((reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(inv_freq)) % 4)
+      return fail(EXL3_ERR_INVALID, "exl3_head_norm: positions and inv_freq must be 4-byte aligned");
+  }
+  a.tokens = tokens;
+  a.d = d;
+  a.R = cfg->rotate_dims;
+  a.interleaved = cfg->interleaved != 0;
+  a.l2 = cfg->mode == EXL3_NORM_L2;
+  a.eps = cfg->eps;
+  a.positions = positions;
+  a.inv_freq = inv_freq;
+  with_elem16(cfg->dtype, [&](auto e) {
+    using E = decltype(e);
+    k_head_norm_any<E><<<dim3((unsigned)tokens, (unsigned)heads), 64, 0, stream_of(stream)>>>(a);
+  });
+  EXL3_LAUNCHED("k_head_norm");
+  return EXL3_OK;
+}

@@ -90,6 +90,38 @@ class HcSite(C.Structure):
                 ("fn", C.c_void_p), ("base", C.c_void_p), ("scale", C.c_void_p)]
 
 
+# exl3_norm_mode
+NORM_RMS = 0
+NORM_L2 = 1
+
+
+class HeadNormConfig(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("mode", C.c_int32), ("head_dim", C.c_int32), ("rotate_dims", C.c_int32),
+                ("interleaved", C.c_int32), ("eps", C.c_float)]
+
+
+class HeadRows(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("w", C.c_void_p), ("y", C.c_void_p), ("heads", C.c_int32),
+                ("x_token", C.c_int64), ("x_head", C.c_int64), ("y_token", C.c_int64), ("y_head", C.c_int64)]
+
+
+class DeltaConfig(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("heads_qk", C.c_int32), ("heads_v", C.c_int32), ("dk", C.c_int32),
+                ("dv", C.c_int32), ("channel_decay", C.c_int32), ("scale", C.c_float)]
+
+
+class DeltaRows(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("g", C.c_void_p), ("beta", C.c_void_p),
+                ("out", C.c_void_p), ("q_token", C.c_int64), ("k_token", C.c_int64), ("v_token", C.c_int64),
+                ("g_token", C.c_int64), ("beta_token", C.c_int64), ("out_token", C.c_int64)]
+
+
+class SampleConfig(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float),
+                ("min_p", C.c_float), ("temperatures", C.c_void_p), ("top_ks", C.c_void_p), ("top_ps", C.c_void_p),
+                ("min_ps", C.c_void_p)]
+
+
 vp, i32, i64, sz = C.c_void_p, C.c_int32, C.c_int64, C.c_size_t
 P = C.POINTER
 
@@ -141,6 +173,11 @@ SIGNATURES = {
     "exl3_hc_mix": (C.c_int, [vp, vp, vp, vp, i64, i32, i32, vp, vp]),
     "exl3_moe_block_workspace_size": (sz, [vp, i32, i64]),
     "exl3_moe_block": (C.c_int, [vp, P(HcSite), vp, C.c_float, vp, i64, vp, vp, sz, vp]),
+    "exl3_head_norm": (C.c_int, [P(HeadNormConfig), P(HeadRows), P(HeadRows), i64, vp, vp, vp]),
+    "exl3_delta_workspace_size": (sz, [P(DeltaConfig), i64, i64]),
+    "exl3_delta_rule": (C.c_int, [P(DeltaConfig), P(DeltaRows), i64, vp, i64, vp, i64, vp, vp, vp, sz, vp]),
+    "exl3_sample_workspace_size": (sz, [i64, i64]),
+    "exl3_sample": (C.c_int, [P(SampleConfig), vp, i64, i64, i64, vp, vp, vp, vp, sz, vp]),
 }
 
 _LIB = None

@@ -440,6 +440,108 @@ exl3_status exl3_moe_layer_load_block(exl3_moe_layer_t layer, const char *const 
 /* For a loaded layer: trellis tensors used in place and repacked (0, 0 otherwise). */
 exl3_status exl3_moe_layer_load_info(exl3_moe_layer_t layer, int64_t *in_place, int64_t *repacked);
 
+/* ---------------------------------------------------------------------------------
+ * The token mixer between the qkv and the output projections, and the choice of a token
+ * behind the head: what a decode step does on either side of the trellis linears.
+ * Element types are exl3_st_dtype values.
+ * --------------------------------------------------------------------------------- */
+
+typedef enum {
+  EXL3_NORM_RMS = 0, /* y = x / sqrt(mean(x^2) + eps) * w */
+  EXL3_NORM_L2 = 1   /* y = x / sqrt(sum(x^2) + eps) * w */
+} exl3_norm_mode;
+
+/* rotate_dims: the first values of a head that the position rotates (even; 0 = none), as
+ * pairs (i, i + rotate_dims/2), or (2i, 2i + 1) when interleaved != 0. */
+typedef struct {
+  int32_t dtype;       /* of x, w and y: EXL3_ST_F16 or EXL3_ST_BF16 */
+  int32_t mode;        /* exl3_norm_mode */
+  int32_t head_dim;    /* 1..1024 */
+  int32_t rotate_dims;
+  int32_t interleaved; /* bool */
+  float eps;           /* >= 0 */
+} exl3_head_norm_config;
+
+/* The heads of one side (queries or keys): value i of head h of token t is
+ * x[t * x_token + h * x_head + i] (strides in elements, so a slice of a packed qkv row is
+ * read in place); y likewise. y may be x itself (same strides); otherwise no output may
+ * overlap an input or the other output. */
+typedef struct {
+  const void *x;   /* device */
+  const void *w;   /* device (head_dim), or NULL: ones */
+  void *y;         /* device */
+  int32_t heads;
+  int64_t x_token, x_head, y_token, y_head;
+} exl3_head_rows;
+
+/* The norm of every query and key head, then its rotation by angle positions[t] *
+ * inv_freq[i] (positions i32 (tokens), inv_freq f32 (rotate_dims / 2), device; may be NULL
+ * when rotate_dims is 0): (a, b) -> (a cos - b sin, b cos + a sin). f32 inside (angles f64),
+ * one rounding. k may be NULL: queries alone. */
+exl3_status exl3_head_norm(const exl3_head_norm_config *cfg, const exl3_head_rows *q, const exl3_head_rows *k,
+                           int64_t tokens, const int32_t *positions, const float *inv_freq, exl3_stream_t stream);
+
+/* dk 64 or 128, dv a multiple of 16 up to 256; heads_v a multiple of heads_qk: value head h
+ * takes query and key head h / (heads_v / heads_qk). */
+typedef struct {
+  int32_t dtype;          /* of q, k, v and out: EXL3_ST_F16 or EXL3_ST_BF16 */
+  int32_t heads_qk, heads_v, dk, dv;
+  int32_t channel_decay;  /* 0: g is (tokens, heads_v); else (tokens, heads_v, dk) */
+  float scale;            /* of the outputs, e.g. 1 / sqrt(dk) */
+} exl3_delta_config;
+
+/* Device rows of a call, token strides in elements (a token's heads lie one behind the
+ * other). g is the log of the decay (0 or less; -inf clears), beta the write strength. */
+typedef struct {
+  const void *q, *k;  /* (tokens, heads_qk, dk) */
+  const void *v;      /* (tokens, heads_v, dv) */
+  const float *g;
+  const float *beta;  /* (tokens, heads_v) */
+  void *out;          /* (tokens, heads_v, dv) */
+  int64_t q_token, k_token, v_token, g_token, beta_token, out_token;
+} exl3_delta_rows;
+
+/* The gated delta rule, for every token of every sequence in turn and every head:
+ *   S <- diag(exp(g)) S;  u = beta * (v - S^T k);  S <- S + k u^T;  out = scale * S^T q
+ * Sequence i is the tokens [starts[i], starts[i+1]) (i32 (n_seq + 1), device, not
+ * decreasing; NULL: n_seq sequences of tokens / n_seq); rows outside every sequence are
+ * left as they are. Values outside [0, tokens] are taken as the nearest of its ends.
+ * state is (n_slots, heads_v, dk, dv) f32, 16-byte aligned: sequence i starts from slot
+ * src[i] and leaves its last state in slot dst[i] (i32 (n_seq), device; src NULL: slot i; dst
+ * NULL: as src, in place). A src outside [0, n_slots) starts from zeros, a dst outside is
+ * not stored. A slot that more than one sequence of the call names is read but keeps its old
+ * state, so no call's result depends on which sequence came first. */
+size_t exl3_delta_workspace_size(const exl3_delta_config *cfg, int64_t tokens, int64_t n_seq);
+exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows *x, int64_t tokens,
+                            const int32_t *starts, int64_t n_seq, float *state, int64_t n_slots, const int32_t *src,
+                            const int32_t *dst, void *workspace, size_t workspace_bytes, exl3_stream_t stream);
+
+/* Each filter's value for every row, or (device arrays of one value a row) for each. */
+typedef struct {
+  int32_t dtype;               /* of the logits: EXL3_ST_F16, EXL3_ST_BF16 or EXL3_ST_F32 */
+  float temperature;           /* <= 0: the largest logit */
+  int32_t top_k;               /* <= 0: all */
+  float top_p;                 /* >= 1: all */
+  float min_p;                 /* <= 0: all */
+  const float *temperatures;   /* (rows) or NULL */
+  const int32_t *top_ks;       /* (rows) or NULL */
+  const float *top_ps;         /* (rows) or NULL */
+  const float *min_ps;         /* (rows) or NULL */
+} exl3_sample_config;
+
+/* One token for each row of logits (rows, vocab; row_stride elements from row to row) from
+ * u[row] in [0, 1). A row is ordered by logit, largest first, equal ones by lower id, with
+ * weights w = exp((logit - largest) / temperature). Kept are the first top_k; of those the
+ * fewest that hold top_p of their weight; of those the ones with w >= min_p; always the
+ * first. ids[row] is the first of the order whose running weight exceeds u times the kept
+ * weight, probs[row] (may be NULL) its share of the kept weight. Logits of -inf or NaN are
+ * never taken; a row of nothing else gets id -1 and probability 0. +inf logits share a row
+ * evenly. Weights under 2^-45 count as 0. At most 65,535 rows of 524,288. */
+size_t exl3_sample_workspace_size(int64_t rows, int64_t vocab);
+exl3_status exl3_sample(const exl3_sample_config *cfg, const void *logits, int64_t rows, int64_t vocab,
+                        int64_t row_stride, const float *u, int32_t *ids, float *probs, void *workspace,
+                        size_t workspace_bytes, exl3_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

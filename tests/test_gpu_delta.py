@@ -1,0 +1,206 @@
+"""GPU tests of exl3_delta_rule against the rule token by token in 64 bits (tolerance derived
+in mixer_cases.check_delta)."""
+import math
+
+import pytest
+import torch
+
+from exl3_amd._lib import Exl3Error
+from exl3_amd.delta import delta_rule
+from mixer_cases import check_delta, delta64, delta_inputs, gen, normal
+
+pytestmark = pytest.mark.gpu
+
+
+def starts_of(lens, first=0):
+    s = [first]
+    for n in lens:
+        s.append(s[-1] + n)
+    return s
+
+
+def ints(v, dev):
+    return torch.tensor(v, device=dev, dtype=torch.int32)
+
+
+def run(dev, lens, Hk=2, Hv=2, dk=128, dv=128, channel=True, dtype=torch.float16, packed=False, seed=0, first=0, tail=0,
+        src=None, dst=None, n_slots=None, change=None, scale=None):
+    starts = starts_of(lens, first)
+    n = len(lens)
+    n_slots = n + 2 if n_slots is None else n_slots
+    x = delta_inputs(seed, dev, starts[-1] + tail, Hk, Hv, dk, dv, channel, n_slots, dtype, packed)
+    if change:
+        change(x)
+    src = [(3 * i + 1) % n_slots if math.gcd(3, n_slots) == 1 else i for i in range(n)] if src is None else src
+    used = src if dst is None else dst
+    sc = dk ** -0.5 if scale is None else scale
+    want, new, size, biggest = delta64(**x, starts=starts, src=src, dst=used, scale=sc)
+    state, was = x["state"].clone(), x["state"].clone()
+    out = torch.full((starts[-1] + tail, Hv, dv), 7.0, device=dev, dtype=dtype)
+    delta_rule(x["q"], x["k"], x["v"], x["g"], x["beta"], state, starts=ints(starts, dev), slots=ints(src, dev),
+               dst=None if dst is None else ints(dst, dev), out=out, scale=scale)
+    # rows outside the sequences stay
+    assert bool((out[:first] == 7).all()) and bool((out[starts[-1]:] == 7).all())
+    check_delta(out, state, want, new, size, biggest, starts, used, dk)
+    written = {used[i] for i in range(n) if not any(used[i] in (src[j], used[j]) for j in range(n) if j != i)}
+    for s in set(range(n_slots)) - written:  # slots that nothing writes keep their bits
+        assert torch.equal(state[s], was[s]), s
+    return x, out, state
+
+
+LENS = [[1], [2], [1, 1, 1], [4, 4], [16], [17], [31], [32], [33], [64], [65], [100, 1, 0, 37], [200], [0, 0, 5], [333, 64, 1, 128]]
+
+
+@pytest.mark.parametrize("lens", LENS, ids=str)
+@pytest.mark.parametrize("channel", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_lengths(dev, lens, channel, dtype):
+    run(dev, lens, channel=channel, dtype=dtype, seed=len(lens))
+
+
+@pytest.mark.parametrize("Hk,Hv,dk,dv", [(1, 1, 64, 16), (3, 3, 64, 64), (2, 4, 128, 48), (1, 5, 128, 96), (4, 4, 64, 256),
+                                         (1, 2, 128, 256), (5, 5, 128, 112)])
+@pytest.mark.parametrize("lens", [[1, 1], [3, 40, 70]], ids=str)
+@pytest.mark.parametrize("channel", [False, True])
+def test_heads_and_sizes(dev, Hk, Hv, dk, dv, lens, channel):
+    run(dev, lens, Hk, Hv, dk, dv, channel, packed=True, seed=Hv + dv, first=2, tail=3)
+
+
+@pytest.mark.parametrize("lens", [[1] * 5, [40, 3, 0, 70, 33]], ids=str)
+def test_slots(dev, lens):
+    n = 5
+    run(dev, lens, src=[4, 3, 2, 1, 0], dst=[5, 6, 7, 8, 9], n_slots=10)           # to other slots
+    run(dev, lens, src=[4, -1, 2, 99, 0], dst=[5, 1, -1, 8, 100], n_slots=10)      # from zeros, and not stored
+    run(dev, lens, src=[1, 1, 2, 3, 4], n_slots=6)                                 # one slot twice: kept
+    run(dev, lens, src=[0, 0, 0, 3, 4], dst=[0, 1, 2, 3, 3], n_slots=6)            # forks; one target twice
+    run(dev, lens, src=[0, 1, 2, 3, 4], dst=[1, 5, 0, 3, 4], n_slots=6)            # a slot that another reads
+    run(dev, lens, src=list(range(n)), n_slots=3)
+
+
+def test_decays_that_clear_and_keep(dev):
+    # g = -inf clears a channel, very negative ones nearly; 0 keeps; chunks and steps agree with the rule
+    def change(x):
+        x["g"][::7] = -math.inf
+        x["g"][3::11] = -500.0
+        x["g"][5::13] = 0.0
+        x["g"][40:] = -1e-4
+        x["g"][60, :, ::2] = -80.0
+    for lens in ([90], [1, 2, 87]):
+        run(dev, lens, channel=True, change=change)
+
+    def change_head(x):
+        x["g"][::7] = -math.inf
+        x["g"][3::11] = -500.0
+        x["g"][5::13] = 0.0
+        x["g"][45:] = -1e-4
+    run(dev, [90], channel=False, change=change_head)
+
+
+def test_strong_and_equal_keys(dev):
+    # the same key over and over with beta 1 replaces the value each time: out = scale v (q = k)
+    def change(x):
+        x["k"][:] = x["k"][:1]
+        x["q"][:] = x["k"]
+        x["beta"][:] = 1.0
+        x["g"][:] = 0.0
+    x, out, _ = run(dev, [75], change=change, scale=1.0)
+    k2 = x["k"][0].double().square().sum(-1)
+    assert float((k2 - 1).abs().max()) < 2e-3  # f16 unit keys
+    assert float((out.double() - x["v"].double()).abs().max()) < 5e-2
+
+    def empty(x):
+        x["beta"][:] = 0.0
+    run(dev, [50], change=empty)
+
+
+def test_special_values_stay_in_their_head_and_sequence(dev):
+    x = delta_inputs(4, dev, 80, 2, 2, 128, 64, True, 2)
+    st = x["state"].clone()
+    clean = delta_rule(x["q"], x["k"], x["v"], x["g"], x["beta"], st, starts=ints([0, 40, 80], dev))
+    v = x["v"].clone()
+    v[50, 1, 3] = math.nan
+    v[60, 1, 9] = math.inf
+    st2 = x["state"].clone()
+    out = delta_rule(x["q"], x["k"], v, x["g"], x["beta"], st2, starts=ints([0, 40, 80], dev))
+    assert torch.equal(out[:40], clean[:40]) and torch.equal(out[:, 0], clean[:, 0]) and torch.equal(st2[0], st[0])
+    assert bool(out[50:, 1, 3].isnan().all()) and torch.equal(out[40:50], clean[40:50])
+    assert torch.equal(out[:, 1, 16:], clean[:, 1, 16:])
+
+
+def test_unordered_starts_stay_in_bounds(dev):
+    # starts that no caller should pass: clamped into the call's tokens, nothing else is touched
+    x = delta_inputs(5, dev, 64, 1, 1, 64, 32, False, 4)
+    buf = torch.zeros((64 + 2, 1, 32), device=dev, dtype=torch.float16)
+    delta_rule(x["q"], x["k"], x["v"], x["g"], x["beta"], x["state"], starts=ints([-7, 50, 20, 1000], dev), out=buf[1:65])
+    assert bool((buf[0] == 0).all()) and bool((buf[65] == 0).all()) and bool(buf.isfinite().all())
+
+
+def test_equal_lengths_without_starts(dev):
+    x = delta_inputs(6, dev, 12, 2, 2, 128, 128, True, 4)
+    a, b = x["state"].clone(), x["state"].clone()
+    slots = ints([2, 0, 3], dev)
+    one = delta_rule(x["q"], x["k"], x["v"], x["g"], x["beta"], a, slots=slots)
+    two = delta_rule(x["q"], x["k"], x["v"], x["g"], x["beta"], b, slots=slots, starts=ints([0, 4, 8, 12], dev))
+    assert torch.equal(one, two) and torch.equal(a, b)
+    a = x["state"].clone()
+    whole = delta_rule(x["q"], x["k"], x["v"], x["g"], x["beta"], a)
+    assert whole.shape == one.shape and torch.equal(a[1:], x["state"][1:])
+
+
+def test_steps_continue_a_prefill(dev):
+    # a prefill and then single tokens give what the whole sequence gives
+    x = delta_inputs(7, dev, 140, 2, 4, 128, 128, True, 1)
+    whole = x["state"].clone()
+    out = delta_rule(x["q"], x["k"], x["v"], x["g"], x["beta"], whole)
+    part = x["state"].clone()
+    outs = []
+    cut = [0, 100, 101, 102, 106, 140]
+    for a, b in zip(cut, cut[1:]):
+        outs.append(delta_rule(*(x[n][a:b] for n in ("q", "k", "v", "g", "beta")), part))
+    want, new, size, biggest = delta64(**x, starts=[0, 140], src=[0], dst=[0], scale=128 ** -0.5)
+    check_delta(out, whole, want, new, size, biggest, [0, 140], [0], 128)
+    check_delta(torch.cat(outs), part, want, new, size, biggest, [0, 140], [0], 128)
+
+
+def test_nothing_to_do_and_refusals(dev):
+    x = delta_inputs(8, dev, 6, 2, 2, 128, 128, True, 3)
+    args = [x[n] for n in ("q", "k", "v", "g", "beta", "state")]
+    was = x["state"].clone()
+    assert delta_rule(*[t[:0] for t in args[:5]], x["state"], starts=ints([0], dev)).shape == (0, 2, 128)
+    delta_rule(*[t[:0] for t in args[:5]], x["state"], starts=ints([0, 0, 0], dev))
+    assert torch.equal(was, x["state"])
+    with pytest.raises(Exl3Error, match="overlap"):
+        delta_rule(*args, out=x["v"])
+    with pytest.raises(ValueError, match="divide"):
+        delta_rule(*args, slots=ints([0, 1, 2, 0], dev))
+
+
+@pytest.mark.parametrize("lens", [[1] * 6, [70, 3, 33]], ids=str)
+def test_graph_replays_and_repeats(dev, lens):
+    starts = starts_of(lens)
+    n = len(lens)
+    x = delta_inputs(9, dev, starts[-1], 2, 2, 128, 128, True, n)
+    st, sl = ints(starts, dev), ints(list(range(n)), dev)
+    out = torch.empty_like(x["v"])
+    from exl3_amd import _lib
+    from exl3_amd.delta import _config
+    need = _lib.lib().exl3_delta_workspace_size(_lib.C.byref(_config(x["q"], x["v"], x["g"], None)), starts[-1], n)
+    ws = torch.empty(max(need, 256), device=dev, dtype=torch.uint8)
+    call = lambda state: delta_rule(x["q"], x["k"], x["v"], x["g"], x["beta"], state, starts=st, slots=sl, out=out, ws=ws)  # noqa: E731
+    live, eager = x["state"].clone(), x["state"].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(live)
+    torch.cuda.current_stream().wait_stream(side)
+    live.copy_(eager)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(live)
+    for i in range(4):
+        x["v"].copy_(normal(gen(90 + i, dev), x["v"].shape, torch.float16))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        call(eager)  # the states carry on from call to call on both sides
+        assert torch.equal(got, out) and torch.equal(live, eager), i
