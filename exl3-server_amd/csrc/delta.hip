@@ -5,6 +5,16 @@
 //   S <- diag(a) S;  u = beta (v - S^T k);  S <- S + k u^T;  out = scale S^T q
 //
 //  k_delta_step   token by token: the state in registers from its slot to its slot.
+//  k_delta_chunk, k_delta_scan   chunks of C = 32 tokens. With the chunk's first state S0, the
+//    running products P_i = a_1 .. a_i and U the rows u of the rule:
+//      A_ij = k_i . (P_i / P_j) k_j (j < i),  B_ij = q_i . (P_i / P_j) k_j (j <= i)
+//      U = T (V - (P K) S0),  T = (I + diag(beta) A)^-1 diag(beta)
+//      out = scale ((P Q) S0 + B U),  S <- diag(P_C) S0 + (P_C / P K)^T U
+//    k_delta_chunk computes T and B of every chunk and head side by side; k_delta_scan goes
+//    through a sequence's chunks with its state in registers.
+//
+// A ratio P_i / P_j is never a quotient nor a difference of sums of g: it is the product
+// of the decays between, which stays exact where a decay is 0 (g = -inf) or tiny.
 #include <hip/hip_runtime.h>
 
 #include <string>
@@ -32,6 +42,7 @@ struct DeltaArgs {
   float *state;
   int64_t n_slots;
   const int32_t *src, *dst;
+  float *chunks;  // (chunk ids, heads_v, kChunkFloats)
 };
 
 struct Seq {
@@ -144,6 +155,389 @@ __global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a) {
       *reinterpret_cast<f32x4 *>(a.state + to * a.heads_v * head + at + (size_t)r * a.dv) = S[r];
 }
 
+// --- chunks ---------------------------------------------------------------------------
+
+constexpr int kC = 32;               // tokens of a chunk
+constexpr int kChunkFloats = 2 * kC * kC + 4;  // T, B and a flag, in the workspace
+constexpr int kPad = 4;              // words behind an LDS row: 16-byte reads of 16 rows meet no bank twice
+
+// Chunk c of sequence i has id first / C + i + c: distinct over the call, under tokens / C + n_seq.
+__device__ __forceinline__ int first_chunk(const Seq &s, int i) { return s.first / kC + i; }
+__device__ __forceinline__ int chunks_of(const Seq &s) { return (s.last - s.first + kC - 1) / kC; }
+
+// The channels a lane holds (DK / 64) of the 8 tokens that its wave holds, and their decays'
+// running products in blocks of `h` tokens: up to and with token i (P), and behind it (X).
+template <typename E, int DK, bool kChannel>
+struct Slice {
+  static constexpr int N = DK / 64;
+  float k[8][N], q[8][N], P[8][N], X[8][N];
+  bool fine;  // no value is infinite or NaN
+
+  // tokens t0 + 8 wave ..; those from `last` on are zeros with decay 1
+  __device__ __forceinline__ void load(const DeltaArgs &a, int t0, int last, int h, int hk) {
+    const int lane = threadIdx.x & 63, first = t0 + (threadIdx.x >> 6) * 8;
+    const E *kp = reinterpret_cast<const E *>(a.k) + (int64_t)hk * DK + lane * N;
+    const E *qp = reinterpret_cast<const E *>(a.q) + (int64_t)hk * DK + lane * N;
+    const float *gp = a.g + (kChannel ? (int64_t)h * DK + lane * N : h);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t t = first + i;
+      const bool on = t < last;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        k[i][n] = on ? to_f32(kp[t * a.k_token + n]) : 0.0f;
+        q[i][n] = on ? to_f32(qp[t * a.q_token + n]) : 0.0f;
+        P[i][n] = on ? gp[t * a.g_token + (kChannel ? n : 0)] : 0.0f;
+      }
+    }
+  }
+  __device__ __forceinline__ void decays() {
+    float z = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        P[i][n] = expf(P[i][n]);
+        X[i][n] = 1.0f;
+        z = fmaf(0.0f, k[i][n], fmaf(0.0f, q[i][n], fmaf(0.0f, P[i][n], z)));
+      }
+    fine = z == 0.0f;
+  }
+  // from blocks of h to blocks of 2 h tokens (h = 1, 2, 4)
+  __device__ __forceinline__ void grow(int h) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int b = i & ~(2 * h - 1);
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (!(i & h)) X[i][n] *= P[b + 2 * h - 1][n];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int b = i & ~(2 * h - 1);
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (i & h) P[i][n] *= P[b + h - 1][n];
+    }
+  }
+};
+
+template <int N>
+__device__ __forceinline__ void put(float *p, const float (&v)[N]) {
+  if constexpr (N == 2) *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]);
+  else *p = v[0];
+}
+template <int N>
+__device__ __forceinline__ void put_scaled(float *p, const float (&v)[N], const float (&s)[N]) {
+  float x[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) x[n] = v[n] * s[n];
+  put<N>(p, x);
+}
+
+__device__ __forceinline__ f32x4 mfma4(const f32x4 &a, const f32x4 &b, f32x4 c) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+
+// T and B of one chunk and value head. For each h = 1, 2, 4, 8, 16 the pairs (i, j) whose
+// highest differing bit is h: i in the later half of a block of 2 h tokens, j in the earlier
+// one, so P_i / P_j = (product from the halves' border to i) (product from j to the border),
+// both at most 1 for decays that are. The 16 rows with bit h and the 16 without it are one
+// tile of the matrix instruction, of which the pairs of a common block are taken.
+template <typename E, int DK, bool kChannel>
+__global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a) {
+  constexpr int N = DK / 64, kRow = DK + kPad;
+  __shared__ float left_k[16 * kRow], left_q[16 * kRow], right[16 * kRow];
+  __shared__ float total[4][DK];
+  __shared__ float sum[2][5][256];             // the second halves of the channels
+  __shared__ float A[kC][kC + kPad], B[kC][kC + kPad];
+  __shared__ float beta[kC], diag[kC];
+  __shared__ int seq;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, id = blockIdx.x, h = blockIdx.y;
+  if (tid == 0) seq = a.n_seq;
+  __syncthreads();
+  for (int i = tid; i < a.n_seq; i += 256) {
+    const Seq s = seq_of(a, i);
+    const int c = id - first_chunk(s, i);
+    if (c >= 0 && c < chunks_of(s)) atomicMin(&seq, i);
+  }
+  __syncthreads();
+  if (seq == a.n_seq) return;
+  const Seq s = seq_of(a, seq);
+  const int t0 = s.first + (id - first_chunk(s, seq)) * kC;
+  Slice<E, DK, kChannel> x;
+  x.load(a, t0, s.last, h, h / (a.heads_v / a.heads_qk));
+  float b = 0.0f;
+  if (tid < kC) {
+    b = t0 + tid < s.last ? a.beta[(int64_t)(t0 + tid) * a.beta_token + h] : 0.0f;
+    beta[tid] = b;
+  }
+  x.decays();
+  const bool fine = !__syncthreads_or(!x.fine || !(b * 0.0f == 0.0f));
+  // B's diagonal
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float d = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n) d = fmaf(x.q[i][n], x.k[i][n], d);
+    d += xor_lanes<1>(d);
+    d += xor_lanes<2>(d);
+    d += xor_lanes<4>(d);
+    d += xor_lanes<8>(d);
+    d += xor_lanes<16>(d);
+    d += xor_lanes<32>(d);
+    if (lane == 0) diag[8 * wave + i] = d;
+  }
+  f32x4 acc[5];
+#pragma unroll
+  for (int level = 0; level < 5; ++level) {
+    const int hh = 1 << level;
+    if (level) __syncthreads();  // the tile's last operands are read
+    if (hh < 8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = (8 * wave + i) / (2 * hh) * hh + (i & (hh - 1));  // without bit h
+        float *at = (i & hh ? left_k : right) + row * kRow + lane * N;
+        if (i & hh) {
+          put_scaled<N>(at, x.k[i], x.P[i]);
+          put_scaled<N>(left_q + row * kRow + lane * N, x.q[i], x.P[i]);
+        } else {
+          put_scaled<N>(at, x.k[i], x.X[i]);
+        }
+      }
+    } else {
+      const bool later = wave & (hh / 8);
+      const int first = hh == 8 ? wave / 2 * 8 : wave % 2 * 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (later) {
+          put_scaled<N>(left_k + (first + i) * kRow + lane * N, x.k[i], x.P[i]);
+          put_scaled<N>(left_q + (first + i) * kRow + lane * N, x.q[i], x.P[i]);
+        } else {
+          put_scaled<N>(right + (first + i) * kRow + lane * N, x.k[i], x.X[i]);
+        }
+      }
+    }
+    if (hh < 8) x.grow(hh);
+    if (hh == 4) put<N>(&total[wave][lane * N], x.P[7]);
+    __syncthreads();
+    // waves 0, 1: A and B over the first half of the channels, waves 2, 3 over the second
+    const float *l = (wave & 1 ? left_q : left_k) + lane % 16 * kRow + lane / 16 * 4;
+    const float *r = right + lane % 16 * kRow + lane / 16 * 4;
+    f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int kt = 0; kt < DK / 32; ++kt) {
+      const int k0 = (wave >> 1) * (DK / 2) + 16 * kt;
+      c = mfma4(*reinterpret_cast<const f32x4 *>(l + k0), *reinterpret_cast<const f32x4 *>(r + k0), c);
+    }
+    acc[level] = c;
+    if (hh == 8) {  // to blocks of 16
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const float t = total[wave ^ 1][lane * N + n];
+          if (wave & 1) x.P[i][n] *= t;
+          else x.X[i][n] *= t;
+        }
+    }
+  }
+  if (wave >= 2) {
+#pragma unroll
+    for (int level = 0; level < 5; ++level)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum[wave & 1][level][r * 64 + lane] = acc[level][r];
+  }
+  for (int i = tid; i < kC * kC; i += 256) {  // on and over the diagonal
+    const int row = i / kC, col = i % kC;
+    if (col >= row) A[row][col] = 0.0f, B[row][col] = col == row ? diag[row] : 0.0f;
+  }
+  __syncthreads();
+  if (wave < 2) {
+    float(*to)[kC + kPad] = wave ? B : A;
+#pragma unroll
+    for (int level = 0; level < 5; ++level)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int hh = 1 << level, ic = lane / 16 * 4 + r, jc = lane % 16;
+        const int i = ic / hh * 2 * hh + hh + ic % hh, j = jc / hh * 2 * hh + jc % hh;
+        if (ic / hh == jc / hh) to[i][j] = acc[level][r] + sum[wave][level][r * 64 + lane];
+      }
+  }
+  __syncthreads();
+  float *out = a.chunks + ((size_t)id * a.heads_v + h) * kChunkFloats;
+  if (wave == 0 && lane < kC) {
+    // column `lane` of T by forward substitution
+    float t[kC];
+#pragma unroll
+    for (int i = 0; i < kC; ++i) {
+      float v = 0.0f;
+#pragma unroll
+      for (int l = 0; l < i; ++l) v = fmaf(A[i][l], t[l], v);
+      t[i] = beta[i] * ((i == lane ? 1.0f : 0.0f) - v);
+      out[i * kC + lane] = t[i];
+    }
+  } else if (wave == 1) {
+    for (int i = lane; i < kC * kC; i += 64) out[kC * kC + i] = B[i / kC][i % kC];
+    if (lane == 0) out[2 * kC * kC] = fine ? 1.0f : 0.0f;
+  }
+}
+
+// A sequence's chunks in turn; a wave holds kCols columns of the state as the accumulators of
+// DK / 16 tiles: lane l column l % 16, rows 16 kt + 4 (l / 16) + r. The same registers are the
+// right operand of the products with the state: instruction j takes element j of each lane's
+// four adjacent rows, and the left operand's columns in that order. U and V - (P K) S0 go
+// from result to operand alike, so nothing but the shared left operands passes through LDS.
+template <typename E, int DK, bool kChannel>
+__global__ __launch_bounds__(256) void k_delta_scan(DeltaArgs a) {
+  constexpr int N = DK / 64, kRow = DK + kPad, KT = DK / 16;
+  __shared__ float pk[kC * kRow], pq[kC * kRow];  // -(P K), P Q
+  __shared__ float pe[DK * (kC + kPad)];          // (P_C / P K)^T
+  __shared__ float total[4][DK];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seq = blockIdx.z, h = blockIdx.y;
+  const int hk = h / (a.heads_v / a.heads_qk), g = lane / 16, m = lane % 16;
+  const int64_t from = slot_of(a.src, seq, a.n_slots), to = slot_of(a.dst, seq, a.n_slots);
+  const bool write = sole_writer(a, seq, to);
+  const Seq s = seq_of(a, seq);
+  const int col = (blockIdx.x * 4 + wave) * kCols + m;
+  const bool mine = (blockIdx.x * 4 + wave) * kCols < a.dv;  // waves past dv only stage
+  const size_t head = (size_t)DK * a.dv;
+  f32x4 S[KT];
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      S[kt][r] = mine && from >= 0 ? a.state[(from * a.heads_v + h) * head + (size_t)(16 * kt + 4 * g + r) * a.dv + col]
+                                   : 0.0f;
+  const E *v = reinterpret_cast<const E *>(a.v) + (int64_t)h * a.dv + col;
+  E *out = reinterpret_cast<E *>(a.out) + (int64_t)h * a.dv + col;
+  for (int c = 0; c < chunks_of(s); ++c) {
+    const int t0 = s.first + c * kC;
+    Slice<E, DK, kChannel> x;
+    x.load(a, t0, s.last, h, hk);
+    x.decays();
+    x.grow(1);
+    x.grow(2);
+    x.grow(4);
+    __syncthreads();  // the last chunk's operands are read
+    put<N>(&total[wave][lane * N], x.P[7]);
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      float before = 1.0f, behind = 1.0f;
+      for (int w = 0; w < 4; ++w) {
+        const float t = total[w][lane * N + n];
+        if (w < wave) before *= t;
+        if (w > wave) behind *= t;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x.P[i][n] *= before, x.X[i][n] *= behind;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = 8 * wave + i;
+      float nk[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) nk[n] = -x.k[i][n];
+      put_scaled<N>(pk + row * kRow + lane * N, nk, x.P[i]);
+      put_scaled<N>(pq + row * kRow + lane * N, x.q[i], x.P[i]);
+#pragma unroll
+      for (int n = 0; n < N; ++n) pe[(lane * N + n) * (kC + kPad) + row] = x.k[i][n] * x.X[i][n];
+    }
+    __syncthreads();
+    if (!mine) continue;
+    const float *mat = a.chunks + ((size_t)(first_chunk(s, seq) + c) * a.heads_v + h) * kChunkFloats;
+    f32x4 X[2], U[2], O[2];
+    float z = mat[2 * kC * kC] - 1.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t t = t0 + 16 * i + 4 * g + r;
+        X[i][r] = t < s.last ? to_f32(v[t * a.v_token]) : 0.0f;
+        z = fmaf(0.0f, X[i][r], z);
+      }
+    if (__any(z != 0.0f)) {
+      // something is infinite or NaN: token by token, so that it reaches no earlier token
+      for (int t = t0; t < min(t0 + kC, s.last); ++t) {
+        const E *k = reinterpret_cast<const E *>(a.k) + (int64_t)t * a.k_token + (int64_t)hk * DK;
+        const E *q = reinterpret_cast<const E *>(a.q) + (int64_t)t * a.q_token + (int64_t)hk * DK;
+        const float *gp = a.g + (int64_t)t * a.g_token + (kChannel ? (int64_t)h * DK : h);
+        float dot = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int ch = 16 * kt + 4 * g + r;
+            S[kt][r] *= expf(gp[kChannel ? ch : 0]);
+            dot = fmaf(to_f32(k[ch]), S[kt][r], dot);
+          }
+        dot += xor_lanes<16>(dot);
+        dot += xor_lanes<32>(dot);
+        const float u = a.beta[(int64_t)t * a.beta_token + h] * (to_f32(v[(int64_t)t * a.v_token]) - dot);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int ch = 16 * kt + 4 * g + r;
+            S[kt][r] = fmaf(to_f32(k[ch]), u, S[kt][r]);
+            o = fmaf(to_f32(q[ch]), S[kt][r], o);
+          }
+        o += xor_lanes<16>(o);
+        o += xor_lanes<32>(o);
+        if (g == 0) out[(int64_t)t * a.out_token] = from_f32<E>(a.scale * o);
+      }
+      continue;
+    }
+    auto operand = [&](const float *p, int stride, int row, int k0) {
+      return *reinterpret_cast<const f32x4 *>(p + (row + m) * stride + k0 + 4 * g);
+    };
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      O[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        X[i] = mfma4(operand(pk, kRow, 16 * i, 16 * kt), S[kt], X[i]);
+        O[i] = mfma4(operand(pq, kRow, 16 * i, 16 * kt), S[kt], O[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      U[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int l = 0; l <= i; ++l) U[i] = mfma4(operand(mat, kC, 16 * i, 16 * l), X[l], U[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int l = 0; l <= i; ++l) O[i] = mfma4(operand(mat + kC * kC, kC, 16 * i, 16 * l), U[l], O[i]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t t = t0 + 16 * i + 4 * g + r;
+        if (t < s.last) out[t * a.out_token] = from_f32<E>(a.scale * O[i][r]);
+      }
+    }
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int ch = 16 * kt + 4 * g + r;
+        S[kt][r] *= total[0][ch] * total[1][ch] * total[2][ch] * total[3][ch];
+      }
+#pragma unroll
+      for (int l = 0; l < 2; ++l) S[kt] = mfma4(operand(pe, kC + kPad, 16 * kt, 16 * l), U[l], S[kt]);
+    }
+  }
+  if (write && mine)
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        a.state[(to * a.heads_v + h) * head + (size_t)(16 * kt + 4 * g + r) * a.dv + col] = S[kt][r];
+}
+
 // f(DK, channel) as compile-time values.
 template <typename F>
 void with_form(int dk, bool channel, F &&f) {
@@ -169,6 +563,15 @@ exl3_status check_config(const exl3_delta_config *c) {
   return EXL3_OK;
 }
 
+// Whether a call goes in chunks: by the sequences' mean length, as their lengths are on the
+// device.
+bool in_chunks(int64_t tokens, int64_t n_seq) { return tokens >= 16 * n_seq; }
+int64_t chunk_ids(int64_t tokens, int64_t n_seq) { return tokens / kC + n_seq; }
+size_t chunk_bytes(const exl3_delta_config *c, int64_t tokens, int64_t n_seq) {
+  return n_seq && in_chunks(tokens, n_seq)
+             ? exl3h::align_up((size_t)chunk_ids(tokens, n_seq) * c->heads_v * kChunkFloats * 4, 256) : 0;
+}
+
 bool bad_counts(int64_t tokens, int64_t n_seq) {
   return tokens < 0 || tokens > ((int64_t)1 << 30) || n_seq < 0 || n_seq > 65535;
 }
@@ -181,7 +584,7 @@ extern "C" {
 
 size_t exl3_delta_workspace_size(const exl3_delta_config *cfg, int64_t tokens, int64_t n_seq) {
   if (check_config(cfg) || bad_counts(tokens, n_seq)) return 0;
-  return 0;
+  return chunk_bytes(cfg, tokens, n_seq);
 }
 
 exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows *x, int64_t tokens,
@@ -220,6 +623,11 @@ exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows 
     if ((i != 3 && spans_meet(x->out, span(3, 2), rows[i], span(i, i < 4 ? 2 : 4))) ||
         spans_meet(state, state_bytes, rows[i], span(i, i < 4 ? 2 : 4)))
       return fail(EXL3_ERR_INVALID, "exl3_delta_rule: out and state must not overlap the call's other rows");
+  const size_t need = chunk_bytes(cfg, tokens, n_seq);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(EXL3_ERR_WORKSPACE, "exl3_delta_rule: workspace too small: need " + std::to_string(need) + " bytes");
+  if (need && reinterpret_cast<uintptr_t>(workspace) % 256)
+    return fail(EXL3_ERR_WORKSPACE, "workspace must be 256-byte aligned");
   DeltaArgs a = {};
   a.q = x->q;
   a.k = x->k;
@@ -244,14 +652,23 @@ exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows 
   a.n_slots = n_slots;
   a.src = src;
   a.dst = dst ? dst : src;
+  a.chunks = reinterpret_cast<float *>(workspace);
   with_elem16(cfg->dtype, [&](auto e) {
     using E = decltype(e);
     with_form(cfg->dk, cfg->channel_decay != 0, [&](auto dk, auto channel) {
+      constexpr int DK = decltype(dk)::value;
+      constexpr bool kChannel = decltype(channel)::value;
+      const hipStream_t st = stream_of(stream);
       const dim3 grid((unsigned)((cfg->dv / kCols + 3) / 4), (unsigned)cfg->heads_v, (unsigned)n_seq);
-      k_delta_step<E, decltype(dk)::value, decltype(channel)::value><<<grid, 256, 0, stream_of(stream)>>>(a);
+      if (need) {
+        k_delta_chunk<E, DK, kChannel><<<dim3((unsigned)chunk_ids(tokens, n_seq), (unsigned)cfg->heads_v), 256, 0, st>>>(a);
+        k_delta_scan<E, DK, kChannel><<<grid, 256, 0, st>>>(a);
+      } else {
+        k_delta_step<E, DK, kChannel><<<grid, 256, 0, st>>>(a);
+      }
     });
   });
-  EXL3_LAUNCHED("k_delta_step");
+  EXL3_LAUNCHED("k_delta");
   return EXL3_OK;
 }
 

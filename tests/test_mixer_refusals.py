@@ -84,7 +84,12 @@ def test_delta_rule_refusals():
     for bad in (dict(out=0x12000000), dict(out=0x10000000 + 100), dict(v=0x20000000), dict(out=0x20000000 + 64)):
         assert delta(x=with_(ROWS, **bad)) == INVALID and b"overlap" in _lib.lib().exl3_last_error(), bad
     assert delta(n=0) == _lib.EXL3_OK
-    assert _lib.lib().exl3_delta_workspace_size(C.byref(with_(DELTA, dk=32)), 64, 2) == 0
+    size = _lib.lib().exl3_delta_workspace_size
+    assert size(C.byref(with_(DELTA, dk=32)), 64, 2) == 0
+    # prefills need a workspace, single tokens none
+    need = size(C.byref(DELTA), 64, 2)
+    assert need > 0 and size(C.byref(DELTA), 64, 64) == 0
+    assert delta(nbytes=need - 1) == delta(ws=None) == delta(ws=0x30000080) == WORKSPACE
 
 
 SAMPLE = SampleConfig(dtype=0, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
