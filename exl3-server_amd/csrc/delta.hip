@@ -31,6 +31,8 @@ namespace {
 
 constexpr int kCols = 16;  // state columns of a wave
 
+struct ChunkMats;
+
 struct DeltaArgs {
   const void *q, *k, *v;
   const float *g, *beta;
@@ -42,7 +44,7 @@ struct DeltaArgs {
   float *state;
   int64_t n_slots;
   const int32_t *src, *dst;
-  float *chunks;  // (chunk ids, heads_v, kChunkFloats)
+  ChunkMats *chunks;  // (chunk ids, heads_v)
 };
 
 struct Seq {
@@ -158,27 +160,48 @@ __global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a) {
 // --- chunks ---------------------------------------------------------------------------
 
 constexpr int kC = 32;               // tokens of a chunk
-constexpr int kChunkFloats = 2 * kC * kC + 4;  // T, B and a flag, in the workspace
-constexpr int kPad = 4;              // words behind an LDS row: 16-byte reads of 16 rows meet no bank twice
+constexpr int kPad = 4;              // words behind an f32 LDS row: 16-byte reads of 16 rows meet no bank twice
+
+// The scan multiplies f16 pairs: x = hi + lo, hi = f16(x), lo = f16(x - hi), 22 bits of x, and
+// three of the four products (lo lo is under 2^-22 of the result). Keys, queries, T and B
+// go in times 2^6, so that the lo of a unit key's values is no subnormal; state columns and
+// the rows between by a power of two that brings the column's largest value to 2^13.
+// A chunk whose values lie outside (|k|, |q|, |T|, |B| under 2^9, decays at most 1) is done
+// token by token in f32.
+constexpr float kScale = 64.0f, kLimit = 512.0f;
+// Of one chunk and head, in the workspace: T and B as hi and lo, the columns in operand order,
+// and two marks of a chunk that the scan may multiply.
+struct ChunkMats {
+  f16 mat[4][kC][kC];  // T hi, T lo, B hi, B lo
+  int32_t fine[4];     // [0], [1] used
+};
+static_assert(sizeof(ChunkMats) % 16 == 0, "16-byte loads");
+// Where the instruction's k index i (of 32) is in operand order: lane group g takes the indices
+// 4 g .. 4 g + 3 and 16 + 4 g .., which are the rows that a result's lane group holds.
+__device__ __forceinline__ constexpr int in_order(int i) {
+  return (i & 12) * 2 + (i & 3) + (i >> 4 & 1) * 4 + (i & ~31);
+}
+
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+struct Pair {
+  f16x8 hi, lo;
+};
 
 // Chunk c of sequence i has id first / C + i + c: distinct over the call, under tokens / C + n_seq.
 __device__ __forceinline__ int first_chunk(const Seq &s, int i) { return s.first / kC + i; }
 __device__ __forceinline__ int chunks_of(const Seq &s) { return (s.last - s.first + kC - 1) / kC; }
 
-// The channels a lane holds (DK / 64) of the 8 tokens that its wave holds, and their decays'
-// running products in blocks of `h` tokens: up to and with token i (P), and behind it (X).
+// The DK / 64 channels of 8 tokens that a lane holds, and their decays' running products in blocks of `h` tokens: up to and with token i (P), and behind it (X).
 template <typename E, int DK, bool kChannel>
 struct Slice {
   static constexpr int N = DK / 64;
   float k[8][N], q[8][N], P[8][N], X[8][N];
-  bool fine;  // no value is infinite or NaN
 
-  // tokens t0 + 8 wave ..; those from `last` on are zeros with decay 1
-  __device__ __forceinline__ void load(const DeltaArgs &a, int t0, int last, int h, int hk) {
-    const int lane = threadIdx.x & 63, first = t0 + (threadIdx.x >> 6) * 8;
-    const E *kp = reinterpret_cast<const E *>(a.k) + (int64_t)hk * DK + lane * N;
-    const E *qp = reinterpret_cast<const E *>(a.q) + (int64_t)hk * DK + lane * N;
-    const float *gp = a.g + (kChannel ? (int64_t)h * DK + lane * N : h);
+  // channels ch .., tokens first ..; those from `last` on are zeros with decay 1
+  __device__ __forceinline__ void load(const DeltaArgs &a, int ch, int first, int last, int h, int hk) {
+    const E *kp = reinterpret_cast<const E *>(a.k) + (int64_t)hk * DK + ch;
+    const E *qp = reinterpret_cast<const E *>(a.q) + (int64_t)hk * DK + ch;
+    const float *gp = a.g + (kChannel ? (int64_t)h * DK + ch : h);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int64_t t = first + i;
@@ -192,16 +215,22 @@ struct Slice {
     }
   }
   __device__ __forceinline__ void decays() {
-    float z = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int n = 0; n < N; ++n) {
         P[i][n] = expf(P[i][n]);
         X[i][n] = 1.0f;
-        z = fmaf(0.0f, k[i][n], fmaf(0.0f, q[i][n], fmaf(0.0f, P[i][n], z)));
       }
-    fine = z == 0.0f;
+  }
+  // Whether the scan may multiply these values (neither does any NaN pass).
+  __device__ __forceinline__ bool fine() const {
+    bool ok = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int n = 0; n < N; ++n) ok = ok && fabsf(k[i][n]) < kLimit && fabsf(q[i][n]) < kLimit && P[i][n] <= 1.0f;
+    return ok;
   }
   // from blocks of h to blocks of 2 h tokens (h = 1, 2, 4)
   __device__ __forceinline__ void grow(int h) {
@@ -268,14 +297,14 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a) {
   const Seq s = seq_of(a, seq);
   const int t0 = s.first + (id - first_chunk(s, seq)) * kC;
   Slice<E, DK, kChannel> x;
-  x.load(a, t0, s.last, h, h / (a.heads_v / a.heads_qk));
+  x.load(a, lane * N, t0 + 8 * wave, s.last, h, h / (a.heads_v / a.heads_qk));
   float b = 0.0f;
   if (tid < kC) {
     b = t0 + tid < s.last ? a.beta[(int64_t)(t0 + tid) * a.beta_token + h] : 0.0f;
     beta[tid] = b;
   }
   x.decays();
-  const bool fine = !__syncthreads_or(!x.fine || !(b * 0.0f == 0.0f));
+  const bool fine = !__syncthreads_or(!x.fine() || !(b * 0.0f == 0.0f));
   // B's diagonal
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -367,42 +396,201 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a) {
       }
   }
   __syncthreads();
-  float *out = a.chunks + ((size_t)id * a.heads_v + h) * kChunkFloats;
-  if (wave == 0 && lane < kC) {
+  ChunkMats &out = a.chunks[(size_t)id * a.heads_v + h];
+  auto put_split = [&](int which, int i, int j, float v) {
+    const float y = f32_rounded(v * kScale);
+    const f16 hi = (f16)y;
+    out.mat[which][i][in_order(j)] = hi;
+    out.mat[which + 1][i][in_order(j)] = (f16)(y - (float)hi);
+  };
+  if (wave == 0) {
     // column `lane` of T by forward substitution
-    float t[kC];
+    float t[kC], most = 0.0f;
+    if (lane < kC) {
 #pragma unroll
-    for (int i = 0; i < kC; ++i) {
-      float v = 0.0f;
+      for (int i = 0; i < kC; ++i) {
+        float v = 0.0f;
 #pragma unroll
-      for (int l = 0; l < i; ++l) v = fmaf(A[i][l], t[l], v);
-      t[i] = beta[i] * ((i == lane ? 1.0f : 0.0f) - v);
-      out[i * kC + lane] = t[i];
+        for (int l = 0; l < i; ++l) v = fmaf(A[i][l], t[l], v);
+        t[i] = beta[i] * ((i == lane ? 1.0f : 0.0f) - v);
+        most = fmaxf(most, fabsf(t[i]));
+        put_split(0, i, lane, t[i]);
+      }
     }
+    const bool large = __any(!(most < kLimit));
+    if (lane == 0) out.fine[0] = fine && !large;
   } else if (wave == 1) {
-    for (int i = lane; i < kC * kC; i += 64) out[kC * kC + i] = B[i / kC][i % kC];
-    if (lane == 0) out[2 * kC * kC] = fine ? 1.0f : 0.0f;
+    float most = 0.0f;
+    for (int i = lane; i < kC * kC; i += 64) {
+      const float v = B[i / kC][i % kC];
+      most = fmaxf(most, fabsf(v));
+      put_split(2, i / kC, i % kC, v);
+    }
+    const bool large = __any(!(most < kLimit));
+    if (lane == 0) out.fine[1] = !large;
   }
 }
 
-// A sequence's chunks in turn; a wave holds kCols columns of the state as the accumulators of
-// DK / 16 tiles: lane l column l % 16, rows 16 kt + 4 (l / 16) + r. The same registers are the
-// right operand of the products with the state: instruction j takes element j of each lane's
-// four adjacent rows, and the left operand's columns in that order. U and V - (P K) S0 go
-// from result to operand alike, so nothing but the shared left operands passes through LDS.
+// One chunk's left operands in LDS, rows in operand order, and the decay over the chunk.
+template <int DK>
+struct alignas(16) Stage {
+  static constexpr int kRow = DK + 8, kTok = kC + 8;  // f16; 16-byte reads of 16 rows meet no bank twice
+  f16 pk[2][kC][kRow], pq[2][kC][kRow];  // P K, P Q: hi, lo
+  f16 pe[2][DK][kTok];                   // (P_C / P K)^T
+  f16 mat[4][kC][kTok];                  // T hi, T lo, B hi, B lo
+  float decay[DK];
+  int fine;
+};
+
+// A power of two that brings the largest of a column's values (lanes l, l ^ 16, l ^ 32, ..) to
+// [2^13, 2^14), and its inverse. 0, denormals and what is not finite take the nearest that exists.
+struct ColumnScale {
+  float to, back;
+  __device__ __forceinline__ explicit ColumnScale(float most) {
+    most = fmaxf(most, xor_lanes<16>(most));
+    most = fmaxf(most, xor_lanes<32>(most));
+    const uint32_t e = max(bitcast<uint32_t>(most) >> 23, 14u);
+    to = bitcast<float>((267u - e) << 23);
+    back = bitcast<float>((e - 13u) << 23);
+  }
+};
+
+__device__ __forceinline__ float most_of(const f32x4 &v, float m) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) m = fmaxf(m, fabsf(v[r]));
+  return m;
+}
+
+// Two tiles' results as a right operand (k index in operand order).
+__device__ __forceinline__ Pair split(const f32x4 &a, const f32x4 &b, float scale) {
+  Pair p;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const float x = f32_rounded(a[r] * scale), y = f32_rounded(b[r] * scale);
+    p.hi[r] = (f16)x;
+    p.hi[4 + r] = (f16)y;
+    p.lo[r] = (f16)(x - (float)p.hi[r]);
+    p.lo[4 + r] = (f16)(y - (float)p.hi[4 + r]);
+  }
+  return p;
+}
+
+__device__ __forceinline__ f32x4 mfma_pair(const Pair &a, const Pair &b, f32x4 c) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.lo, b.hi, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.lo, c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.hi, c, 0, 0, 0);
+}
+
+// N adjacent scaled values as f16 pairs. (The values are products: rounded to f32 first, or
+// hi could be the product rounded once to f16 in one place and twice in the other, and lo
+// the rest of neither.)
+template <int N>
+__device__ __forceinline__ void put_split(f16 *hi, f16 *lo, const float (&v)[N]) {
+  f16 h[N], l[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const float x = f32_rounded(v[n]);
+    h[n] = (f16)x;
+    l[n] = (f16)(x - (float)h[n]);
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) hi[n] = h[n], lo[n] = l[n];
+}
+
+// A sequence's chunks in turn. Waves 0 to 3 hold kCols columns of the state each, as the
+// accumulators of DK / 16 tiles: lane l column l % 16, rows 16 kt + 4 (l / 16) + r. As the rows
+// of a result are taken for the k indices of the next product (`in_order`), the state,
+// V - (P K) S0 and U go from result to right operand within the lane; only the left operands,
+// which all waves share, pass through LDS. Waves 4 to 7 prepare the next chunk's there, in
+// the other of two buffers, and load the one after it.
 template <typename E, int DK, bool kChannel>
-__global__ __launch_bounds__(256) void k_delta_scan(DeltaArgs a) {
-  constexpr int N = DK / 64, kRow = DK + kPad, KT = DK / 16;
-  __shared__ float pk[kC * kRow], pq[kC * kRow];  // -(P K), P Q
-  __shared__ float pe[DK * (kC + kPad)];          // (P_C / P K)^T
-  __shared__ float total[4][DK];
+__global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a) {
+  constexpr int N = DK / 64, KT = DK / 16;
+  __shared__ Stage<DK> stage[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seq = blockIdx.z, h = blockIdx.y;
   const int hk = h / (a.heads_v / a.heads_qk), g = lane / 16, m = lane % 16;
   const int64_t from = slot_of(a.src, seq, a.n_slots), to = slot_of(a.dst, seq, a.n_slots);
   const bool write = sole_writer(a, seq, to);
   const Seq s = seq_of(a, seq);
+  const int chunks = chunks_of(s);
+  const ChunkMats *mats = a.chunks + (size_t)first_chunk(s, seq) * a.heads_v + h;
+
+  if (wave >= 4) {
+    // lane: channels ch .. of tokens 8 g ..
+    const int ch = (wave - 4) * (DK / 4) + m * N;
+    Slice<E, DK, kChannel> x;
+    u32x4 mat[2];
+    int fine[2];
+    auto load = [&](int c) {
+      x.load(a, ch, s.first + c * kC + 8 * g, s.last, h, hk);
+      const ChunkMats &in = mats[(size_t)c * a.heads_v];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        mat[i] = reinterpret_cast<const u32x4 *>(in.mat)[(tid - 256) + 256 * i];
+      fine[0] = in.fine[0];
+      fine[1] = in.fine[1];
+    };
+    auto prepare = [&](Stage<DK> &st) {
+      x.decays();
+      x.grow(1);
+      x.grow(2);
+      x.grow(4);
+      float all[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        // products of the 8 tokens of the other lane groups, before and behind this one's
+        const float own = x.P[7][n], o1 = xor_lanes<16>(own), two = own * o1, o2 = xor_lanes<32>(two);
+        const float before = (g & 1 ? o1 : 1.0f) * (g & 2 ? o2 : 1.0f);
+        const float behind = (g & 1 ? 1.0f : o1) * (g & 2 ? 1.0f : o2);
+        all[n] = two * o2;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x.P[i][n] *= before * kScale, x.X[i][n] *= behind * kScale;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = 8 * g + i, col = in_order(ch);
+        float pk[N], pq[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) pk[n] = x.k[i][n] * x.P[i][n], pq[n] = x.q[i][n] * x.P[i][n];
+        put_split<N>(&st.pk[0][row][col], &st.pk[1][row][col], pk);
+        put_split<N>(&st.pq[0][row][col], &st.pq[1][row][col], pq);
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+          const int at = in_order(8 * g + i);
+          float pe[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) pe[j] = x.k[i + j][n] * x.X[i + j][n];
+          put_split<4>(&st.pe[0][ch + n][at], &st.pe[1][ch + n][at], pe);
+        }
+      if (g == 0) put<N>(&st.decay[ch], all);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = (tid - 256) + 256 * i;  // of 512 pieces of 8 values: 4 matrices of 32 rows of 4
+        *reinterpret_cast<u32x4 *>(&st.mat[at / 128][at / 4 % 32][at % 4 * 8]) = mat[i];
+      }
+      if (tid == 256) st.fine = fine[0] && fine[1];
+    };
+    if (chunks > 0) {
+      load(0);
+      prepare(stage[0]);
+      if (chunks > 1) load(1);
+    }
+    __syncthreads();
+    for (int c = 0; c < chunks; ++c) {
+      if (c + 1 < chunks) {
+        prepare(stage[(c + 1) & 1]);
+        if (c + 2 < chunks) load(c + 2);
+      }
+      __syncthreads();
+    }
+    return;
+  }
+
   const int col = (blockIdx.x * 4 + wave) * kCols + m;
-  const bool mine = (blockIdx.x * 4 + wave) * kCols < a.dv;  // waves past dv only stage
+  const bool mine = (blockIdx.x * 4 + wave) * kCols < a.dv;  // waves past dv only keep step
   const size_t head = (size_t)DK * a.dv;
   f32x4 S[KT];
 #pragma unroll
@@ -413,54 +601,34 @@ __global__ __launch_bounds__(256) void k_delta_scan(DeltaArgs a) {
                                    : 0.0f;
   const E *v = reinterpret_cast<const E *>(a.v) + (int64_t)h * a.dv + col;
   E *out = reinterpret_cast<E *>(a.out) + (int64_t)h * a.dv + col;
-  for (int c = 0; c < chunks_of(s); ++c) {
-    const int t0 = s.first + c * kC;
-    Slice<E, DK, kChannel> x;
-    x.load(a, t0, s.last, h, hk);
-    x.decays();
-    x.grow(1);
-    x.grow(2);
-    x.grow(4);
-    __syncthreads();  // the last chunk's operands are read
-    put<N>(&total[wave][lane * N], x.P[7]);
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      float before = 1.0f, behind = 1.0f;
-      for (int w = 0; w < 4; ++w) {
-        const float t = total[w][lane * N + n];
-        if (w < wave) before *= t;
-        if (w > wave) behind *= t;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x.P[i][n] *= before, x.X[i][n] *= behind;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int row = 8 * wave + i;
-      float nk[N];
-#pragma unroll
-      for (int n = 0; n < N; ++n) nk[n] = -x.k[i][n];
-      put_scaled<N>(pk + row * kRow + lane * N, nk, x.P[i]);
-      put_scaled<N>(pq + row * kRow + lane * N, x.q[i], x.P[i]);
-#pragma unroll
-      for (int n = 0; n < N; ++n) pe[(lane * N + n) * (kC + kPad) + row] = x.k[i][n] * x.X[i][n];
-    }
-    __syncthreads();
-    if (!mine) continue;
-    const float *mat = a.chunks + ((size_t)(first_chunk(s, seq) + c) * a.heads_v + h) * kChunkFloats;
-    f32x4 X[2], U[2], O[2];
-    float z = mat[2 * kC * kC] - 1.0f;
+  float next_v[2][4];
+  auto load_v = [&](int c) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int64_t t = t0 + 16 * i + 4 * g + r;
-        X[i][r] = t < s.last ? to_f32(v[t * a.v_token]) : 0.0f;
-        z = fmaf(0.0f, X[i][r], z);
+        const int64_t t = s.first + c * kC + 16 * i + 4 * g + r;
+        next_v[i][r] = mine && t < s.last ? to_f32(v[t * a.v_token]) : 0.0f;
       }
-    if (__any(z != 0.0f)) {
-      // something is infinite or NaN: token by token, so that it reaches no earlier token
+  };
+  load_v(0);
+  __syncthreads();
+  for (int c = 0; c < chunks; ++c, __syncthreads()) {
+    const int t0 = s.first + c * kC;
+    const Stage<DK> &st = stage[c & 1];
+    if (!mine) continue;
+    f32x4 V[2];
+    float z = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        V[i][r] = next_v[i][r];
+        z = fmaf(0.0f, V[i][r], z);
+      }
+    load_v(c + 1);
+    if (!st.fine || __any(z != 0.0f)) {
+      // something is infinite, NaN or out of range: token by token, so that it reaches no earlier token
       for (int t = t0; t < min(t0 + kC, s.last); ++t) {
         const E *k = reinterpret_cast<const E *>(a.k) + (int64_t)t * a.k_token + (int64_t)hk * DK;
         const E *q = reinterpret_cast<const E *>(a.q) + (int64_t)t * a.q_token + (int64_t)hk * DK;
@@ -491,43 +659,60 @@ __global__ __launch_bounds__(256) void k_delta_scan(DeltaArgs a) {
       }
       continue;
     }
-    auto operand = [&](const float *p, int stride, int row, int k0) {
-      return *reinterpret_cast<const f32x4 *>(p + (row + m) * stride + k0 + 4 * g);
+    auto left = [&](const f16 *hi, const f16 *lo) {
+      return Pair{*reinterpret_cast<const f16x8 *>(hi + 8 * g), *reinterpret_cast<const f16x8 *>(lo + 8 * g)};
     };
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    float most = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      O[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int kt = 0; kt < KT; ++kt) most = most_of(S[kt], most);
+    const ColumnScale ss(most);
+    f32x4 X[2] = {zero, zero}, O[2] = {zero, zero}, W[2];
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        X[i] = mfma4(operand(pk, kRow, 16 * i, 16 * kt), S[kt], X[i]);
-        O[i] = mfma4(operand(pq, kRow, 16 * i, 16 * kt), S[kt], O[i]);
+    for (int u = 0; u < KT / 2; ++u) {
+      const Pair right = split(S[2 * u], S[2 * u + 1], ss.to);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        X[i] = mfma_pair(left(&st.pk[0][16 * i + m][32 * u], &st.pk[1][16 * i + m][32 * u]), right, X[i]);
+        O[i] = mfma_pair(left(&st.pq[0][16 * i + m][32 * u], &st.pq[1][16 * i + m][32 * u]), right, O[i]);
       }
     }
+    const float cs = ss.back / kScale;
+    most = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      U[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int l = 0; l <= i; ++l) U[i] = mfma4(operand(mat, kC, 16 * i, 16 * l), X[l], U[i]);
+      for (int r = 0; r < 4; ++r) X[i][r] = fmaf(-cs, X[i][r], V[i][r]);
+      most = most_of(X[i], most);
     }
+    const ColumnScale sx(most);
+    const Pair x = split(X[0], X[1], sx.to);
+    most = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
+      W[i] = mfma_pair(left(st.mat[0][16 * i + m], st.mat[1][16 * i + m]), x, zero);
 #pragma unroll
-      for (int l = 0; l <= i; ++l) O[i] = mfma4(operand(mat + kC * kC, kC, 16 * i, 16 * l), U[l], O[i]);
+      for (int r = 0; r < 4; ++r) W[i][r] *= sx.back / kScale;
+      most = most_of(W[i], most);
+    }
+    const ColumnScale su(most);
+    const Pair u = split(W[0], W[1], su.to);
+    const float cu = su.back / kScale;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const f32x4 bu = mfma_pair(left(st.mat[2][16 * i + m], st.mat[3][16 * i + m]), u, zero);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int64_t t = t0 + 16 * i + 4 * g + r;
-        if (t < s.last) out[t * a.out_token] = from_f32<E>(a.scale * O[i][r]);
+        if (t < s.last) out[t * a.out_token] = from_f32<E>(a.scale * fmaf(cs, O[i][r], cu * bu[r]));
       }
     }
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
+      const f32x4 add = mfma_pair(left(st.pe[0][16 * kt + m], st.pe[1][16 * kt + m]), u, zero);
+      const f32x4 d = *reinterpret_cast<const f32x4 *>(&st.decay[16 * kt + 4 * g]);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int ch = 16 * kt + 4 * g + r;
-        S[kt][r] *= total[0][ch] * total[1][ch] * total[2][ch] * total[3][ch];
-      }
-#pragma unroll
-      for (int l = 0; l < 2; ++l) S[kt] = mfma4(operand(pe, kC + kPad, 16 * kt, 16 * l), U[l], S[kt]);
+      for (int r = 0; r < 4; ++r) S[kt][r] = fmaf(cu, add[r], d[r] * S[kt][r]);
     }
   }
   if (write && mine)
@@ -569,7 +754,7 @@ bool in_chunks(int64_t tokens, int64_t n_seq) { return tokens >= 16 * n_seq; }
 int64_t chunk_ids(int64_t tokens, int64_t n_seq) { return tokens / kC + n_seq; }
 size_t chunk_bytes(const exl3_delta_config *c, int64_t tokens, int64_t n_seq) {
   return n_seq && in_chunks(tokens, n_seq)
-             ? exl3h::align_up((size_t)chunk_ids(tokens, n_seq) * c->heads_v * kChunkFloats * 4, 256) : 0;
+             ? exl3h::align_up((size_t)chunk_ids(tokens, n_seq) * c->heads_v * sizeof(ChunkMats), 256) : 0;
 }
 
 bool bad_counts(int64_t tokens, int64_t n_seq) {
@@ -652,7 +837,7 @@ exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows 
   a.n_slots = n_slots;
   a.src = src;
   a.dst = dst ? dst : src;
-  a.chunks = reinterpret_cast<float *>(workspace);
+  a.chunks = reinterpret_cast<ChunkMats *>(workspace);
   with_elem16(cfg->dtype, [&](auto e) {
     using E = decltype(e);
     with_form(cfg->dk, cfg->channel_decay != 0, [&](auto dk, auto channel) {
@@ -662,7 +847,7 @@ exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows 
       const dim3 grid((unsigned)((cfg->dv / kCols + 3) / 4), (unsigned)cfg->heads_v, (unsigned)n_seq);
       if (need) {
         k_delta_chunk<E, DK, kChannel><<<dim3((unsigned)chunk_ids(tokens, n_seq), (unsigned)cfg->heads_v), 256, 0, st>>>(a);
-        k_delta_scan<E, DK, kChannel><<<grid, 256, 0, st>>>(a);
+        k_delta_scan<E, DK, kChannel><<<grid, 512, 0, st>>>(a);
       } else {
         k_delta_step<E, DK, kChannel><<<grid, 256, 0, st>>>(a);
       }

@@ -123,7 +123,13 @@ def test_special_values_stay_in_their_head_and_sequence(dev):
     st2 = x["state"].clone()
     out = delta_rule(x["q"], x["k"], v, x["g"], x["beta"], st2, starts=ints([0, 40, 80], dev))
     assert torch.equal(out[:40], clean[:40]) and torch.equal(out[:, 0], clean[:, 0]) and torch.equal(st2[0], st[0])
-    assert bool(out[50:, 1, 3].isnan().all()) and torch.equal(out[40:50], clean[40:50])
+    # the tokens before it: the rule's values (a chunk with a NaN goes token by token, so the last
+    # bits of its 16 columns' outputs may differ from the clean call's)
+    part = {n: t[:50] if n != "state" else t for n, t in x.items()}
+    want, new, size, biggest = delta64(**part, starts=[0, 40, 50], src=[0, 1], dst=[0, 1], scale=128 ** -0.5)
+    bound = (2.0 ** -11 * (1 + 2.0 ** -10) * want.abs() + 2.0 ** -25
+             + 8 * math.sqrt(144 * 11) * 2.0 ** -24 * size[..., None])  # check_delta's for 10 tokens
+    assert bool(out[50:, 1, 3].isnan().all()) and bool(((out[40:50].double() - want[40:]).abs() <= bound[40:]).all())
     assert torch.equal(out[:, 1, 16:], clean[:, 1, 16:])
 
 
