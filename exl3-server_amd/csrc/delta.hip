@@ -191,37 +191,76 @@ struct Pair {
 __device__ __forceinline__ int first_chunk(const Seq &s, int i) { return s.first / kC + i; }
 __device__ __forceinline__ int chunks_of(const Seq &s) { return (s.last - s.first + kC - 1) / kC; }
 
-// The DK / 64 channels of 8 tokens that a lane holds, and their decays' running products in blocks of `h` tokens: up to and with token i (P), and behind it (X).
+// exp(g). (The product's rounding costs |g| 2^-24 of a factor exp(g): at most 2^-25.)
+__device__ __forceinline__ float decay_of(float g) { return __builtin_amdgcn_exp2f(g * 1.44269504f); }
+
+// A uniform value that the compiler cannot see to be one.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// The first of a chunk's rows of `stride` elements of E, at head offset `at` (uniform).
+template <typename E>
+__device__ __forceinline__ const char *chunk_rows(const void *p, int64_t stride, int t0, int64_t at) {
+  return reinterpret_cast<const char *>(p) + (t0 * stride + at) * (int64_t)sizeof(E);
+}
+
+// The DK / 64 channels of 8 tokens that a lane holds, as they lie in memory: loaded a chunk
+// ahead and converted when they are taken, so that no load is waited for one by one. Tokens
+// behind the chunk's n read its last row's values, which convert() clears.
+template <typename E, int DK, bool kChannel>
+struct RawSlice {
+  static constexpr int N = DK / 64, G = kChannel ? N : 1;
+  typedef E EN __attribute__((ext_vector_type(N), aligned(2)));
+  typedef float GN __attribute__((ext_vector_type(G), aligned(4)));
+  EN k[8], q[8];
+  GN g[8];
+
+  // chunk tokens tok .., channels ch ..
+  __device__ __forceinline__ void load(const DeltaArgs &a, int t0, int n, int h, int hk, int tok, int ch) {
+    const char *kb = chunk_rows<E>(a.k, a.k_token, t0, (int64_t)hk * DK);
+    const char *qb = chunk_rows<E>(a.q, a.q_token, t0, (int64_t)hk * DK);
+    const char *gb = chunk_rows<float>(a.g, a.g_token, t0, kChannel ? (int64_t)h * DK : h);
+    const uint32_t ks = (uint32_t)a.k_token * 2, qs = (uint32_t)a.q_token * 2, gs = (uint32_t)a.g_token * 4;
+    const uint32_t c2 = ch * 2, c4 = kChannel ? ch * 4 : 0;
+    if (n >= kC) {
+      const uint32_t ko = tok * ks + c2, qo = tok * qs + c2, go = tok * gs + c4;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        k[i] = *reinterpret_cast<const EN *>(kb + (size_t)i * ks + ko);
+        q[i] = *reinterpret_cast<const EN *>(qb + (size_t)i * qs + qo);
+        g[i] = *reinterpret_cast<const GN *>(gb + (size_t)i * gs + go);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t t = min(tok + i, n - 1);
+        k[i] = *reinterpret_cast<const EN *>(kb + (t * ks + c2));
+        q[i] = *reinterpret_cast<const EN *>(qb + (t * qs + c2));
+        g[i] = *reinterpret_cast<const GN *>(gb + (t * gs + c4));
+      }
+    }
+  }
+};
+
+// The same in f32, and the decays' running products in blocks of `h` tokens: up to and with
+// token i (P), and behind it (X).
 template <typename E, int DK, bool kChannel>
 struct Slice {
   static constexpr int N = DK / 64;
   float k[8][N], q[8][N], P[8][N], X[8][N];
 
-  // channels ch .., tokens first ..; those from `last` on are zeros with decay 1
-  __device__ __forceinline__ void load(const DeltaArgs &a, int ch, int first, int last, int h, int hk) {
-    const E *kp = reinterpret_cast<const E *>(a.k) + (int64_t)hk * DK + ch;
-    const E *qp = reinterpret_cast<const E *>(a.q) + (int64_t)hk * DK + ch;
-    const float *gp = a.g + (kChannel ? (int64_t)h * DK + ch : h);
+  // blocks of one token; tokens from n on are zeros with decay 1
+  __device__ __forceinline__ void convert(const RawSlice<E, DK, kChannel> &x, int n, int tok) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int64_t t = first + i;
-      const bool on = t < last;
+      const bool on = tok + i < n;
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        k[i][n] = on ? to_f32(kp[t * a.k_token + n]) : 0.0f;
-        q[i][n] = on ? to_f32(qp[t * a.q_token + n]) : 0.0f;
-        P[i][n] = on ? gp[t * a.g_token + (kChannel ? n : 0)] : 0.0f;
+      for (int c = 0; c < N; ++c) {
+        k[i][c] = on ? to_f32((E)x.k[i][c]) : 0.0f;
+        q[i][c] = on ? to_f32((E)x.q[i][c]) : 0.0f;
+        P[i][c] = on ? decay_of(x.g[i][kChannel ? c : 0]) : 1.0f;
+        X[i][c] = 1.0f;
       }
     }
-  }
-  __device__ __forceinline__ void decays() {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        P[i][n] = expf(P[i][n]);
-        X[i][n] = 1.0f;
-      }
   }
   // Whether the scan may multiply these values (neither does any NaN pass).
   __device__ __forceinline__ bool fine() const {
@@ -295,15 +334,16 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a) {
   __syncthreads();
   if (seq == a.n_seq) return;
   const Seq s = seq_of(a, seq);
-  const int t0 = s.first + (id - first_chunk(s, seq)) * kC;
-  Slice<E, DK, kChannel> x;
-  x.load(a, lane * N, t0 + 8 * wave, s.last, h, h / (a.heads_v / a.heads_qk));
+  const int t0 = uniform(s.first + (id - first_chunk(s, seq)) * kC), n = uniform(s.last) - t0;
+  RawSlice<E, DK, kChannel> raw;
+  raw.load(a, t0, n, h, h / (a.heads_v / a.heads_qk), 8 * wave, lane * N);
   float b = 0.0f;
   if (tid < kC) {
-    b = t0 + tid < s.last ? a.beta[(int64_t)(t0 + tid) * a.beta_token + h] : 0.0f;
+    b = tid < n ? a.beta[(int64_t)(t0 + tid) * a.beta_token + h] : 0.0f;
     beta[tid] = b;
   }
-  x.decays();
+  Slice<E, DK, kChannel> x;
+  x.convert(raw, n, 8 * wave);
   const bool fine = !__syncthreads_or(!x.fine() || !(b * 0.0f == 0.0f));
   // B's diagonal
 #pragma unroll
@@ -431,6 +471,14 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a) {
   }
 }
 
+// A barrier that orders LDS alone: __syncthreads() would also wait for every global load and
+// store in flight, which here are the next chunk's.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // One chunk's left operands in LDS, rows in operand order, and the decay over the chunk.
 template <int DK>
 struct alignas(16) Stage {
@@ -511,18 +559,20 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a) {
   const int hk = h / (a.heads_v / a.heads_qk), g = lane / 16, m = lane % 16;
   const int64_t from = slot_of(a.src, seq, a.n_slots), to = slot_of(a.dst, seq, a.n_slots);
   const bool write = sole_writer(a, seq, to);
-  const Seq s = seq_of(a, seq);
+  Seq s = seq_of(a, seq);
+  s = Seq{uniform(s.first), uniform(s.last)};
   const int chunks = chunks_of(s);
   const ChunkMats *mats = a.chunks + (size_t)first_chunk(s, seq) * a.heads_v + h;
 
   if (wave >= 4) {
     // lane: channels ch .. of tokens 8 g ..
     const int ch = (wave - 4) * (DK / 4) + m * N;
-    Slice<E, DK, kChannel> x;
+    RawSlice<E, DK, kChannel> raw;
     u32x4 mat[2];
     int fine[2];
     auto load = [&](int c) {
-      x.load(a, ch, s.first + c * kC + 8 * g, s.last, h, hk);
+      const int t0 = s.first + c * kC;
+      raw.load(a, t0, s.last - t0, h, hk, 8 * g, ch);
       const ChunkMats &in = mats[(size_t)c * a.heads_v];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -530,8 +580,10 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a) {
       fine[0] = in.fine[0];
       fine[1] = in.fine[1];
     };
-    auto prepare = [&](Stage<DK> &st) {
-      x.decays();
+    auto prepare = [&](int c) {
+      Stage<DK> &st = stage[c & 1];
+      Slice<E, DK, kChannel> x;
+      x.convert(raw, s.last - (s.first + c * kC), 8 * g);
       x.grow(1);
       x.grow(2);
       x.grow(4);
@@ -575,16 +627,16 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a) {
     };
     if (chunks > 0) {
       load(0);
-      prepare(stage[0]);
+      prepare(0);
       if (chunks > 1) load(1);
     }
-    __syncthreads();
+    lds_barrier();
     for (int c = 0; c < chunks; ++c) {
       if (c + 1 < chunks) {
-        prepare(stage[(c + 1) & 1]);
+        prepare(c + 1);
         if (c + 2 < chunks) load(c + 2);
       }
-      __syncthreads();
+      lds_barrier();
     }
     return;
   }
@@ -601,20 +653,25 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a) {
                                    : 0.0f;
   const E *v = reinterpret_cast<const E *>(a.v) + (int64_t)h * a.dv + col;
   E *out = reinterpret_cast<E *>(a.out) + (int64_t)h * a.dv + col;
-  float next_v[2][4];
+  // the next chunk's values as they lie in memory (behind its tokens: the last one's)
+  E next_v[2][4];
+  const int64_t v_at = mine ? (int64_t)h * a.dv + col : 0;
   auto load_v = [&](int c) {
+    const int t0 = s.first + c * kC, n = s.last - t0;
+    const char *vb = chunk_rows<E>(a.v, a.v_token, t0, 0);
+    const uint32_t vs = (uint32_t)a.v_token * 2;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int64_t t = s.first + c * kC + 16 * i + 4 * g + r;
-        next_v[i][r] = mine && t < s.last ? to_f32(v[t * a.v_token]) : 0.0f;
+        const uint32_t t = min(16 * i + 4 * g + r, n - 1);
+        next_v[i][r] = *reinterpret_cast<const E *>(vb + (t * vs + (uint32_t)v_at * 2));
       }
   };
-  load_v(0);
-  __syncthreads();
-  for (int c = 0; c < chunks; ++c, __syncthreads()) {
-    const int t0 = s.first + c * kC;
+  if (chunks > 0) load_v(0);
+  lds_barrier();
+  for (int c = 0; c < chunks; ++c, lds_barrier()) {
+    const int t0 = s.first + c * kC, n = s.last - t0;
     const Stage<DK> &st = stage[c & 1];
     if (!mine) continue;
     f32x4 V[2];
@@ -623,10 +680,10 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a) {
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        V[i][r] = next_v[i][r];
+        V[i][r] = 16 * i + 4 * g + r < n ? to_f32(next_v[i][r]) : 0.0f;
         z = fmaf(0.0f, V[i][r], z);
       }
-    load_v(c + 1);
+    if (c + 1 < chunks) load_v(c + 1);
     if (!st.fine || __any(z != 0.0f)) {
       // something is infinite, NaN or out of range: token by token, so that it reaches no earlier token
       for (int t = t0; t < min(t0 + kC, s.last); ++t) {
@@ -639,7 +696,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int ch = 16 * kt + 4 * g + r;
-            S[kt][r] *= expf(gp[kChannel ? ch : 0]);
+            S[kt][r] *= decay_of(gp[kChannel ? ch : 0]);
             dot = fmaf(to_f32(k[ch]), S[kt][r], dot);
           }
         dot += xor_lanes<16>(dot);
@@ -698,13 +755,17 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a) {
     const ColumnScale su(most);
     const Pair u = split(W[0], W[1], su.to);
     const float cu = su.back / kScale;
+    char *ob = const_cast<char *>(chunk_rows<E>(a.out, a.out_token, t0, 0));
+    const uint32_t os = (uint32_t)a.out_token * 2;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const f32x4 bu = mfma_pair(left(st.mat[2][16 * i + m], st.mat[3][16 * i + m]), u, zero);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int64_t t = t0 + 16 * i + 4 * g + r;
-        if (t < s.last) out[t * a.out_token] = from_f32<E>(a.scale * fmaf(cs, O[i][r], cu * bu[r]));
+        const int t = 16 * i + 4 * g + r;
+        if (t < n)
+          *reinterpret_cast<E *>(ob + (uint32_t)(t * os + (uint32_t)v_at * 2)) =
+              from_f32<E>(a.scale * fmaf(cs, O[i][r], cu * bu[r]));
       }
     }
 #pragma unroll
@@ -792,8 +853,9 @@ exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows 
   const int64_t strides[6][2] = {{x->q_token, qk}, {x->k_token, qk}, {x->v_token, vo},
                                  {x->out_token, vo}, {x->g_token, gs}, {x->beta_token, cfg->heads_v}};
   for (const auto &s : strides)
-    if (tokens > 1 && (s[0] < s[1] || s[0] > ((int64_t)1 << 31)))
-      return fail(EXL3_ERR_INVALID, "exl3_delta_rule: a token stride is smaller than a token's heads");
+    // (under 2^24 elements, a chunk's rows lie within 32-bit offsets)
+    if (tokens > 1 && (s[0] < s[1] || s[0] >= ((int64_t)1 << 24)))
+      return fail(EXL3_ERR_INVALID, "exl3_delta_rule: a token stride is smaller than a token's heads, or 2^24 or more");
   if ((reinterpret_cast<uintptr_t>(x->q) | reinterpret_cast<uintptr_t>(x->k) | reinterpret_cast<uintptr_t>(x->v) |
        reinterpret_cast<uintptr_t>(x->out)) % 2 ||
       (reinterpret_cast<uintptr_t>(x->g) | reinterpret_cast<uintptr_t>(x->beta) | reinterpret_cast<uintptr_t>(starts) |
