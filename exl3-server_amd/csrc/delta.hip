@@ -225,9 +225,9 @@ struct RawSlice {
       const uint32_t ko = tok * ks + c2, qo = tok * qs + c2, go = tok * gs + c4;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        k[i] = *reinterpret_cast<const EN *>(kb + (size_t)i * ks + ko);
-        q[i] = *reinterpret_cast<const EN *>(qb + (size_t)i * qs + qo);
-        g[i] = *reinterpret_cast<const GN *>(gb + (size_t)i * gs + go);
+        k[i] = *reinterpret_cast<const EN *>(kb + (ko + i * ks));
+        q[i] = *reinterpret_cast<const EN *>(qb + (qo + i * qs));
+        g[i] = *reinterpret_cast<const GN *>(gb + (go + i * gs));
       }
     } else {
 #pragma unroll
@@ -251,15 +251,20 @@ struct Slice {
   // blocks of one token; tokens from n on are zeros with decay 1
   __device__ __forceinline__ void convert(const RawSlice<E, DK, kChannel> &x, int n, int tok) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool on = tok + i < n;
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int c = 0; c < N; ++c) {
-        k[i][c] = on ? to_f32((E)x.k[i][c]) : 0.0f;
-        q[i][c] = on ? to_f32((E)x.q[i][c]) : 0.0f;
-        P[i][c] = on ? decay_of(x.g[i][kChannel ? c : 0]) : 1.0f;
+        k[i][c] = to_f32((E)x.k[i][c]);
+        q[i][c] = to_f32((E)x.q[i][c]);
+        P[i][c] = kChannel || c == 0 ? decay_of(x.g[i][c % RawSlice<E, DK, kChannel>::G]) : P[i][0];
         X[i][c] = 1.0f;
       }
+    if (n < kC) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+          if (tok + i >= n) k[i][c] = q[i][c] = 0.0f, P[i][c] = 1.0f;
     }
   }
   // Whether the scan may multiply these values (neither does any NaN pass).
@@ -480,12 +485,14 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 // One chunk's left operands in LDS, rows in operand order, and the decay over the chunk.
-template <int DK>
+template <typename E, int DK, int kWaves>
 struct alignas(16) Stage {
+  static constexpr int kCol = kWaves * kCols + 8;
   static constexpr int kRow = DK + 8, kTok = kC + 8;  // f16; 16-byte reads of 16 rows meet no bank twice
   f16 pk[2][kC][kRow], pq[2][kC][kRow];  // P K, P Q: hi, lo
   f16 pe[2][DK][kTok];                   // (P_C / P K)^T
   f16 mat[4][kC][kTok];                  // T hi, T lo, B hi, B lo
+  E v[kC][kCol];
   float decay[DK];
   int fine;
 };
@@ -495,8 +502,11 @@ struct alignas(16) Stage {
 struct ColumnScale {
   float to, back;
   __device__ __forceinline__ explicit ColumnScale(float most) {
-    most = fmaxf(most, xor_lanes<16>(most));
-    most = fmaxf(most, xor_lanes<32>(most));
+    // the two exchanges hold each lane's own value and its partner's, in either order
+    const auto r16 = __builtin_amdgcn_permlane16_swap(bitcast<uint32_t>(most), bitcast<uint32_t>(most), false, false);
+    most = fmaxf(bitcast<float>(r16[0]), bitcast<float>(r16[1]));
+    const auto r32 = __builtin_amdgcn_permlane32_swap(bitcast<uint32_t>(most), bitcast<uint32_t>(most), false, false);
+    most = fmaxf(bitcast<float>(r32[0]), bitcast<float>(r32[1]));
     const uint32_t e = max(bitcast<uint32_t>(most) >> 23, 14u);
     to = bitcast<float>((267u - e) << 23);
     back = bitcast<float>((e - 13u) << 23);
@@ -509,52 +519,76 @@ __device__ __forceinline__ float most_of(const f32x4 &v, float m) {
   return m;
 }
 
+// x s and y s as f16 pairs: hi rounded once, lo the rest of it. hi passes through a register
+// that the compiler may not compute twice: a product rounded to f32 first in one place and
+// not in the other would leave a lo that fits neither.
+__device__ __forceinline__ void split2(float x, float xs, float y, float ys, f16x2 &hi, f16x2 &lo) {
+  uint32_t h = bitcast<uint32_t>(f16x2{(f16)(x * xs), (f16)(y * ys)});
+  asm("" : "+v"(h));
+  hi = bitcast<f16x2>(h);
+  lo = f16x2{(f16)fmaf(x, xs, -(float)hi[0]), (f16)fmaf(y, ys, -(float)hi[1])};
+}
+
 // Two tiles' results as a right operand (k index in operand order).
 __device__ __forceinline__ Pair split(const f32x4 &a, const f32x4 &b, float scale) {
+  f16x2 h[4], l[4];
+#pragma unroll
+  for (int r = 0; r < 4; r += 2) {
+    split2(a[r], scale, a[r + 1], scale, h[r / 2], l[r / 2]);
+    split2(b[r], scale, b[r + 1], scale, h[2 + r / 2], l[2 + r / 2]);
+  }
   Pair p;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const float x = f32_rounded(a[r] * scale), y = f32_rounded(b[r] * scale);
-    p.hi[r] = (f16)x;
-    p.hi[4 + r] = (f16)y;
-    p.lo[r] = (f16)(x - (float)p.hi[r]);
-    p.lo[4 + r] = (f16)(y - (float)p.hi[4 + r]);
-  }
+  for (int r = 0; r < 8; ++r) p.hi[r] = h[r / 2][r % 2], p.lo[r] = l[r / 2][r % 2];
   return p;
 }
 
-__device__ __forceinline__ f32x4 mfma_pair(const Pair &a, const Pair &b, f32x4 c) {
-  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.lo, b.hi, c, 0, 0, 0);
-  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.lo, c, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.hi, c, 0, 0, 0);
-}
-
-// N adjacent scaled values as f16 pairs. (The values are products: rounded to f32 first, or
-// hi could be the product rounded once to f16 in one place and twice in the other, and lo
-// the rest of neither.)
-template <int N>
-__device__ __forceinline__ void put_split(f16 *hi, f16 *lo, const float (&v)[N]) {
-  f16 h[N], l[N];
+// c[i] += sum over u of left[u][i] right[u] (lo lo left out), the results' chains in turn.
+template <int U, int R>
+__device__ __forceinline__ void product(const Pair (&left)[U][R], const Pair (&right)[U], f32x4 (&c)[R]) {
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const float x = f32_rounded(v[n]);
-    h[n] = (f16)x;
-    l[n] = (f16)(x - (float)h[n]);
+  for (int u = 0; u < U; ++u) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) c[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(left[u][i].lo, right[u].hi, c[i], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < R; ++i) c[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(left[u][i].hi, right[u].lo, c[i], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < R; ++i) c[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(left[u][i].hi, right[u].hi, c[i], 0, 0, 0);
   }
-#pragma unroll
-  for (int n = 0; n < N; ++n) hi[n] = h[n], lo[n] = l[n];
 }
 
-// A sequence's chunks in turn. Waves 0 to 3 hold kCols columns of the state each, as the
+// N adjacent values v s as f16 pairs.
+template <int N>
+__device__ __forceinline__ void put_split(f16 *hi, f16 *lo, const float (&v)[N], const float (&sc)[N]) {
+  f16x2 h[(N + 1) / 2], l[(N + 1) / 2];
+#pragma unroll
+  for (int n = 0; n < N; n += 2) split2(v[n], sc[n], v[n + 1 < N ? n + 1 : n], sc[n + 1 < N ? n + 1 : n], h[n / 2], l[n / 2]);
+  if constexpr (N == 1) *hi = h[0][0], *lo = l[0][0];
+  else {
+    typedef uint32_t words __attribute__((ext_vector_type(N / 2)));
+    words wh, wl;
+    if constexpr (N == 2) wh = bitcast<uint32_t>(h[0]), wl = bitcast<uint32_t>(l[0]);
+    else {
+#pragma unroll
+      for (int n = 0; n < N / 2; ++n) wh[n] = bitcast<uint32_t>(h[n]), wl[n] = bitcast<uint32_t>(l[n]);
+    }
+    *reinterpret_cast<words *>(hi) = wh;
+    *reinterpret_cast<words *>(lo) = wl;
+  }
+}
+
+// A sequence's chunks in turn. The first kWaves waves hold kCols columns of the state each, as the
 // accumulators of DK / 16 tiles: lane l column l % 16, rows 16 kt + 4 (l / 16) + r. As the rows
 // of a result are taken for the k indices of the next product (`in_order`), the state,
 // V - (P K) S0 and U go from result to right operand within the lane; only the left operands,
-// which all waves share, pass through LDS. Waves 4 to 7 prepare the next chunk's there, in
-// the other of two buffers, and load the one after it.
-template <typename E, int DK, bool kChannel>
-__global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a) {
+// which all waves share, pass through LDS. The four waves behind them prepare the next chunk's
+// there (and its values), in the other of two buffers, and load the one after it: the
+// multiplying waves wait for no load, and their stores are never waited for.
+template <typename E, int DK, bool kChannel, int kWaves>
+__global__ __launch_bounds__(64 * kWaves + 256) void k_delta_scan(DeltaArgs a) {
   constexpr int N = DK / 64, KT = DK / 16;
-  __shared__ Stage<DK> stage[2];
+  using St = Stage<E, DK, kWaves>;
+  __shared__ St stage[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seq = blockIdx.z, h = blockIdx.y;
   const int hk = h / (a.heads_v / a.heads_qk), g = lane / 16, m = lane % 16;
   const int64_t from = slot_of(a.src, seq, a.n_slots), to = slot_of(a.dst, seq, a.n_slots);
@@ -564,24 +598,35 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a) {
   const int chunks = chunks_of(s);
   const ChunkMats *mats = a.chunks + (size_t)first_chunk(s, seq) * a.heads_v + h;
 
-  if (wave >= 4) {
+  if (wave >= kWaves) {
     // lane: channels ch .. of tokens 8 g ..
-    const int ch = (wave - 4) * (DK / 4) + m * N;
+    const int part = tid - 64 * kWaves, ch = part / 64 * (DK / 4) + m * N;
     RawSlice<E, DK, kChannel> raw;
     u32x4 mat[2];
     int fine[2];
+    // 8 values of a row; kPieces such pieces are the workgroup's columns
+    typedef E E8 __attribute__((ext_vector_type(8), aligned(2)));
+    constexpr int kPieces = kWaves * kCols / 8;
+    const uint32_t v_col = blockIdx.x * kWaves * kCols + part % kPieces * 8;
+    const bool has_v = part < kC * kPieces && (int)v_col < a.dv;
+    E8 val;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) val[i] = from_f32<E>(0.0f);
     auto load = [&](int c) {
       const int t0 = s.first + c * kC;
       raw.load(a, t0, s.last - t0, h, hk, 8 * g, ch);
       const ChunkMats &in = mats[(size_t)c * a.heads_v];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        mat[i] = reinterpret_cast<const u32x4 *>(in.mat)[(tid - 256) + 256 * i];
+        mat[i] = reinterpret_cast<const u32x4 *>(in.mat)[part + 256 * i];
       fine[0] = in.fine[0];
       fine[1] = in.fine[1];
+      const uint32_t t = min(part / kPieces, s.last - t0 - 1);
+      const char *vb = chunk_rows<E>(a.v, a.v_token, t0, (int64_t)h * a.dv);
+      if (has_v) val = *reinterpret_cast<const E8 *>(vb + (t * (uint32_t)a.v_token + v_col) * 2);
     };
     auto prepare = [&](int c) {
-      Stage<DK> &st = stage[c & 1];
+      St &st = stage[c & 1];
       Slice<E, DK, kChannel> x;
       x.convert(raw, s.last - (s.first + c * kC), 8 * g);
       x.grow(1);
@@ -601,29 +646,31 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int row = 8 * g + i, col = in_order(ch);
-        float pk[N], pq[N];
-#pragma unroll
-        for (int n = 0; n < N; ++n) pk[n] = x.k[i][n] * x.P[i][n], pq[n] = x.q[i][n] * x.P[i][n];
-        put_split<N>(&st.pk[0][row][col], &st.pk[1][row][col], pk);
-        put_split<N>(&st.pq[0][row][col], &st.pq[1][row][col], pq);
+        put_split<N>(&st.pk[0][row][col], &st.pk[1][row][col], x.k[i], x.P[i]);
+        put_split<N>(&st.pq[0][row][col], &st.pq[1][row][col], x.q[i], x.P[i]);
       }
 #pragma unroll
       for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int i = 0; i < 8; i += 4) {
           const int at = in_order(8 * g + i);
-          float pe[4];
+          float k4[4], x4[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) pe[j] = x.k[i + j][n] * x.X[i + j][n];
-          put_split<4>(&st.pe[0][ch + n][at], &st.pe[1][ch + n][at], pe);
+          for (int j = 0; j < 4; ++j) k4[j] = x.k[i + j][n], x4[j] = x.X[i + j][n];
+          put_split<4>(&st.pe[0][ch + n][at], &st.pe[1][ch + n][at], k4, x4);
         }
       if (g == 0) put<N>(&st.decay[ch], all);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int at = (tid - 256) + 256 * i;  // of 512 pieces of 8 values: 4 matrices of 32 rows of 4
+        const int at = part + 256 * i;  // of 512 pieces of 8 values: 4 matrices of 32 rows of 4
         *reinterpret_cast<u32x4 *>(&st.mat[at / 128][at / 4 % 32][at % 4 * 8]) = mat[i];
       }
-      if (tid == 256) st.fine = fine[0] && fine[1];
+      if (part == 0) st.fine = fine[0] && fine[1];
+      if (part / kPieces >= s.last - (s.first + c * kC)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) val[i] = from_f32<E>(0.0f);
+      }
+      if (part < kC * kPieces) *reinterpret_cast<u32x4 *>(&st.v[part / kPieces][part % kPieces * 8]) = bitcast<u32x4>(val);
     };
     if (chunks > 0) {
       load(0);
@@ -641,99 +688,101 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a) {
     return;
   }
 
-  const int col = (blockIdx.x * 4 + wave) * kCols + m;
-  const bool mine = (blockIdx.x * 4 + wave) * kCols < a.dv;  // waves past dv only keep step
+  const int col = (blockIdx.x * kWaves + wave) * kCols + m;
+  if ((blockIdx.x * kWaves + wave) * kCols >= a.dv) {  // only keeps step
+    for (int c = 0; c <= chunks; ++c) lds_barrier();
+    return;
+  }
   const size_t head = (size_t)DK * a.dv;
   f32x4 S[KT];
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      S[kt][r] = mine && from >= 0 ? a.state[(from * a.heads_v + h) * head + (size_t)(16 * kt + 4 * g + r) * a.dv + col]
-                                   : 0.0f;
+      S[kt][r] = from >= 0 ? a.state[(from * a.heads_v + h) * head + (size_t)(16 * kt + 4 * g + r) * a.dv + col] : 0.0f;
   const E *v = reinterpret_cast<const E *>(a.v) + (int64_t)h * a.dv + col;
   E *out = reinterpret_cast<E *>(a.out) + (int64_t)h * a.dv + col;
-  // the next chunk's values as they lie in memory (behind its tokens: the last one's)
-  E next_v[2][4];
-  const int64_t v_at = mine ? (int64_t)h * a.dv + col : 0;
-  auto load_v = [&](int c) {
-    const int t0 = s.first + c * kC, n = s.last - t0;
-    const char *vb = chunk_rows<E>(a.v, a.v_token, t0, 0);
-    const uint32_t vs = (uint32_t)a.v_token * 2;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint32_t t = min(16 * i + 4 * g + r, n - 1);
-        next_v[i][r] = *reinterpret_cast<const E *>(vb + (t * vs + (uint32_t)v_at * 2));
-      }
-  };
-  if (chunks > 0) load_v(0);
-  lds_barrier();
-  for (int c = 0; c < chunks; ++c, lds_barrier()) {
-    const int t0 = s.first + c * kC, n = s.last - t0;
-    const Stage<DK> &st = stage[c & 1];
-    if (!mine) continue;
-    f32x4 V[2];
+
+  // Whether chunk c may be multiplied, and its values.
+  f32x4 V[2];
+  auto fine_chunk = [&](int c) {
+    const St &st = stage[c & 1];
     float z = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        V[i][r] = 16 * i + 4 * g + r < n ? to_f32(next_v[i][r]) : 0.0f;
+        V[i][r] = to_f32(st.v[16 * i + 4 * g + r][wave * kCols + m]);
         z = fmaf(0.0f, V[i][r], z);
       }
-    if (c + 1 < chunks) load_v(c + 1);
-    if (!st.fine || __any(z != 0.0f)) {
-      // something is infinite, NaN or out of range: token by token, so that it reaches no earlier token
-      for (int t = t0; t < min(t0 + kC, s.last); ++t) {
-        const E *k = reinterpret_cast<const E *>(a.k) + (int64_t)t * a.k_token + (int64_t)hk * DK;
-        const E *q = reinterpret_cast<const E *>(a.q) + (int64_t)t * a.q_token + (int64_t)hk * DK;
-        const float *gp = a.g + (int64_t)t * a.g_token + (kChannel ? (int64_t)h * DK : h);
-        float dot = 0.0f, o = 0.0f;
+    return st.fine && !__any(z != 0.0f);
+  };
+  // Chunk c token by token in f32, where something in it is infinite, NaN or out of range, so
+  // that it reaches no earlier token.
+  auto by_token = [&](int c) {
+    const int t0 = s.first + c * kC;
+    for (int t = t0; t < min(t0 + kC, s.last); ++t) {
+      const E *k = reinterpret_cast<const E *>(a.k) + (int64_t)t * a.k_token + (int64_t)hk * DK;
+      const E *q = reinterpret_cast<const E *>(a.q) + (int64_t)t * a.q_token + (int64_t)hk * DK;
+      const float *gp = a.g + (int64_t)t * a.g_token + (kChannel ? (int64_t)h * DK : h);
+      float dot = 0.0f, o = 0.0f;
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
+      for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int ch = 16 * kt + 4 * g + r;
-            S[kt][r] *= decay_of(gp[kChannel ? ch : 0]);
-            dot = fmaf(to_f32(k[ch]), S[kt][r], dot);
-          }
-        dot += xor_lanes<16>(dot);
-        dot += xor_lanes<32>(dot);
-        const float u = a.beta[(int64_t)t * a.beta_token + h] * (to_f32(v[(int64_t)t * a.v_token]) - dot);
+        for (int r = 0; r < 4; ++r) {
+          const int ch = 16 * kt + 4 * g + r;
+          S[kt][r] *= decay_of(gp[kChannel ? ch : 0]);
+          dot = fmaf(to_f32(k[ch]), S[kt][r], dot);
+        }
+      dot += xor_lanes<16>(dot);
+      dot += xor_lanes<32>(dot);
+      const float u = a.beta[(int64_t)t * a.beta_token + h] * (to_f32(v[(int64_t)t * a.v_token]) - dot);
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
+      for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int ch = 16 * kt + 4 * g + r;
-            S[kt][r] = fmaf(to_f32(k[ch]), u, S[kt][r]);
-            o = fmaf(to_f32(q[ch]), S[kt][r], o);
-          }
-        o += xor_lanes<16>(o);
-        o += xor_lanes<32>(o);
-        if (g == 0) out[(int64_t)t * a.out_token] = from_f32<E>(a.scale * o);
-      }
-      continue;
+        for (int r = 0; r < 4; ++r) {
+          const int ch = 16 * kt + 4 * g + r;
+          S[kt][r] = fmaf(to_f32(k[ch]), u, S[kt][r]);
+          o = fmaf(to_f32(q[ch]), S[kt][r], o);
+        }
+      o += xor_lanes<16>(o);
+      o += xor_lanes<32>(o);
+      if (g == 0) out[(int64_t)t * a.out_token] = from_f32<E>(a.scale * o);
     }
+  };
+  auto multiply = [&](int c) {
+    const int t0 = s.first + c * kC, n = s.last - t0;
+    const St &st = stage[c & 1];
     auto left = [&](const f16 *hi, const f16 *lo) {
       return Pair{*reinterpret_cast<const f16x8 *>(hi + 8 * g), *reinterpret_cast<const f16x8 *>(lo + 8 * g)};
     };
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int UT = KT / 2;
+    // left operands are read well before their products
+    Pair pk[UT][2], pq[UT][2], right[UT];
+#pragma unroll
+    for (int u = 0; u < UT; ++u)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) pk[u][i] = left(&st.pk[0][16 * i + m][32 * u], &st.pk[1][16 * i + m][32 * u]);
+#pragma unroll
+    for (int u = 0; u < UT; ++u)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) pq[u][i] = left(&st.pq[0][16 * i + m][32 * u], &st.pq[1][16 * i + m][32 * u]);
+    __builtin_amdgcn_sched_barrier(0);
     float most = 0.0f;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) most = most_of(S[kt], most);
     const ColumnScale ss(most);
-    f32x4 X[2] = {zero, zero}, O[2] = {zero, zero}, W[2];
 #pragma unroll
-    for (int u = 0; u < KT / 2; ++u) {
-      const Pair right = split(S[2 * u], S[2 * u + 1], ss.to);
+    for (int u = 0; u < UT; ++u) right[u] = split(S[2 * u], S[2 * u + 1], ss.to);
+    f32x4 X[2] = {zero, zero}, O[2] = {zero, zero}, W[2] = {zero, zero}, BU[2] = {zero, zero};
+    product<UT, 2>(pk, right, X);
+    product<UT, 2>(pq, right, O);
+    Pair mt[1][2], mb[1][2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        X[i] = mfma_pair(left(&st.pk[0][16 * i + m][32 * u], &st.pk[1][16 * i + m][32 * u]), right, X[i]);
-        O[i] = mfma_pair(left(&st.pq[0][16 * i + m][32 * u], &st.pq[1][16 * i + m][32 * u]), right, O[i]);
-      }
-    }
+    for (int i = 0; i < 2; ++i) mt[0][i] = left(st.mat[0][16 * i + m], st.mat[1][16 * i + m]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) mb[0][i] = left(st.mat[2][16 * i + m], st.mat[3][16 * i + m]);
     const float cs = ss.back / kScale;
     most = 0.0f;
 #pragma unroll
@@ -743,40 +792,60 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a) {
       most = most_of(X[i], most);
     }
     const ColumnScale sx(most);
-    const Pair x = split(X[0], X[1], sx.to);
+    const Pair x[1] = {split(X[0], X[1], sx.to)};
+    product<1, 2>(mt, x, W);
+    Pair pe[1][KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) pe[0][kt] = left(st.pe[0][16 * kt + m], st.pe[1][16 * kt + m]);
     most = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      W[i] = mfma_pair(left(st.mat[0][16 * i + m], st.mat[1][16 * i + m]), x, zero);
 #pragma unroll
       for (int r = 0; r < 4; ++r) W[i][r] *= sx.back / kScale;
       most = most_of(W[i], most);
     }
     const ColumnScale su(most);
-    const Pair u = split(W[0], W[1], su.to);
+    const Pair u[1] = {split(W[0], W[1], su.to)};
     const float cu = su.back / kScale;
-    char *ob = const_cast<char *>(chunk_rows<E>(a.out, a.out_token, t0, 0));
-    const uint32_t os = (uint32_t)a.out_token * 2;
+    product<1, 2>(mb, u, BU);
+    f32x4 add[KT];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const f32x4 bu = mfma_pair(left(st.mat[2][16 * i + m], st.mat[3][16 * i + m]), u, zero);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = 16 * i + 4 * g + r;
-        if (t < n)
-          *reinterpret_cast<E *>(ob + (uint32_t)(t * os + (uint32_t)v_at * 2)) =
-              from_f32<E>(a.scale * fmaf(cs, O[i][r], cu * bu[r]));
-      }
-    }
+    for (int kt = 0; kt < KT; ++kt) add[kt] = zero;
+    product<1, KT>(pe, u, add);
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-      const f32x4 add = mfma_pair(left(st.pe[0][16 * kt + m], st.pe[1][16 * kt + m]), u, zero);
       const f32x4 d = *reinterpret_cast<const f32x4 *>(&st.decay[16 * kt + 4 * g]);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) S[kt][r] = fmaf(cu, add[r], d[r] * S[kt][r]);
+      for (int r = 0; r < 4; ++r) S[kt][r] = fmaf(cu, add[kt][r], d[r] * S[kt][r]);
     }
+    char *ob = const_cast<char *>(chunk_rows<E>(a.out, a.out_token, t0, (int64_t)h * a.dv));
+    const uint32_t os = (uint32_t)a.out_token * 2, oo = 4 * g * os + col * 2;
+    E o[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[i][r] = from_f32<E>(a.scale * fmaf(cs, O[i][r], cu * BU[i][r]));
+    if (n >= kC) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) *reinterpret_cast<E *>(ob + (oo + (16 * i + r) * os)) = o[i][r];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (16 * i + 4 * g + r < n) *reinterpret_cast<E *>(ob + (oo + (16 * i + r) * os)) = o[i][r];
+    }
+  };
+  lds_barrier();
+  // the rare chunks outside the loop over the others, whose registers and waits they would shape
+  for (int c = 0; c < chunks; ++c, lds_barrier()) {
+    for (; c < chunks && fine_chunk(c); ++c, lds_barrier()) multiply(c);
+    if (c == chunks) break;
+    by_token(c);
   }
-  if (write && mine)
+  if (write)
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -909,7 +978,9 @@ exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows 
       const dim3 grid((unsigned)((cfg->dv / kCols + 3) / 4), (unsigned)cfg->heads_v, (unsigned)n_seq);
       if (need) {
         k_delta_chunk<E, DK, kChannel><<<dim3((unsigned)chunk_ids(tokens, n_seq), (unsigned)cfg->heads_v), 256, 0, st>>>(a);
-        k_delta_scan<E, DK, kChannel><<<grid, 512, 0, st>>>(a);
+        const int waves = 2;
+        const dim3 scan((unsigned)((cfg->dv / kCols + waves - 1) / waves), (unsigned)cfg->heads_v, (unsigned)n_seq);
+        k_delta_scan<E, DK, kChannel, 2><<<scan, 64 * 2 + 256, 0, st>>>(a);
       } else {
         k_delta_step<E, DK, kChannel><<<grid, 256, 0, st>>>(a);
       }
