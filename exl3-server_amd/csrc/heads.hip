@@ -23,6 +23,9 @@ using namespace exl3e;
 namespace {
 
 constexpr int kMaxHeadDim = 1024;
+constexpr int kMaxFastDim = 512;  // 64 lanes of 8 values
+constexpr int kThreads = 256;
+constexpr int kEnough = 2048;     // workgroups: 8 a CU
 
 struct HeadSide {
   const void *x, *w;
@@ -92,6 +95,95 @@ __global__ __launch_bounds__(64) void k_head_norm_any(HeadArgs a) {
 size_t span_bytes(const HeadSide &s, bool out, int64_t T, int d) {
   const int64_t t = out ? s.y_token : s.x_token, h = out ? s.y_head : s.x_head;
   return (size_t)((T - 1) * t + (s.heads - 1) * h + d) * 2;
+}
+
+// Heads of up to 512 values in groups of 8, at 16-byte addresses: kLanes lanes of 8 values each
+// (a power of two; lanes past the head are idle) hold a head in registers, 256 / kLanes heads a
+// workgroup at once. A token's angles are computed once for all of a workgroup's heads, while
+// the first heads' values are on their way. The partners of a rotation by halves are read
+// again (from the first-level cache), which costs less than 8 lane exchanges; a head's lanes are
+// of one wave, whose loads are done before its stores, so that works in place as well.
+// Bound by HBM for many tokens, by latency for few.
+template <typename E, int kLanes>
+__global__ __launch_bounds__(kThreads) void k_head_norm(HeadArgs a, int per_group) {
+  constexpr int kAtOnce = kThreads / kLanes;
+  __shared__ float2 turns[kMaxFastDim / 2];
+  const int64_t tok = blockIdx.x;
+  const int l = threadIdx.x % kLanes, e = 8 * l, half = a.R / 2, all = a.s[0].heads + a.s[1].heads;
+  const int first = blockIdx.y * per_group + threadIdx.x / kLanes, last = min(all, (int)(blockIdx.y + 1) * per_group);
+  // this lane's rotation: of pairs inside it, with the half behind or before it, or none
+  const bool pairs = a.interleaved && e < a.R, later = !a.interleaved && e >= half && e < a.R;
+  const bool halves = !a.interleaved && e < a.R;
+  const int other = later ? e - half : e + half;
+  auto row = [&](int h, const HeadSide *&s, const E *&x) {
+    const bool second = h >= a.s[0].heads;
+    s = &a.s[second];
+    const int hh = second ? h - a.s[0].heads : h;
+    x = reinterpret_cast<const E *>(s->x) + tok * s->x_token + hh * s->x_head;
+    return hh;
+  };
+  float x[8] = {}, p[8] = {};
+  auto fetch = [&](int h) {
+    const HeadSide *s;
+    const E *at;
+    row(h, s, at);
+    if (e < a.d) load8(at + e, x);
+    if (halves) load8(at + other, p);
+  };
+  if (first < last) fetch(first);
+  if (a.R) {
+    const int32_t pos = a.positions[tok];
+    for (int i = threadIdx.x; i < half; i += kThreads) turns[i] = turn(pos, a.inv_freq[i]);
+    __syncthreads();
+  }
+  for (int h = first; h < last; h += kAtOnce) {
+    const HeadSide *s;
+    const E *at;
+    const int hh = row(h, s, at);
+    float sq = 0.0f, y[8], o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      y[i] = x[i];
+      o[i] = p[i];
+      sq = fmaf(x[i], x[i], sq);
+    }
+    if (h + kAtOnce < last) fetch(h + kAtOnce);
+#pragma unroll
+    for (int m = 1; m < kLanes; m <<= 1) sq += __shfl_xor(sq, m);
+    const float r = scale_of(a, sq);
+    const E *w = reinterpret_cast<const E *>(s->w);
+    if (e >= a.d) continue;
+    float wv[8];
+    if (w) load8(w + e, wv);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = y[i] * r * (w ? wv[i] : 1.0f);
+    if (pairs) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        if (e + i < a.R) {
+          const float2 cs = turns[e / 2 + i / 2];
+          const float u = y[i], v = y[i + 1];
+          y[i] = u * cs.x - v * cs.y;
+          y[i + 1] = v * cs.x + u * cs.y;
+        }
+      }
+    } else if (halves) {
+      if (w) load8(w + other, wv);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 cs = turns[(later ? other : e) + i];
+        const float v = o[i] * r * (w ? wv[i] : 1.0f);
+        y[i] = later ? y[i] * cs.x + v * cs.y : y[i] * cs.x - v * cs.y;
+      }
+    }
+    store8(reinterpret_cast<E *>(s->y) + tok * s->y_token + hh * s->y_head + e, y);
+  }
+}
+
+// Whether a side's rows and weights lie at 16-byte addresses.
+bool aligned16(const HeadSide &s) {
+  return (reinterpret_cast<uintptr_t>(s.x) | reinterpret_cast<uintptr_t>(s.y) | reinterpret_cast<uintptr_t>(s.w)) % 16 == 0 &&
+         (s.x_token | s.x_head | s.y_token | s.y_head) % 8 == 0;
 }
 
 // Whether two sides' rows share a value: exactly where both are token-major with one token
@@ -179,7 +271,27 @@ extern "C" exl3_status exl3_head_norm(const exl3_head_norm_config *cfg, const ex
   a.inv_freq = inv_freq;
   with_elem16(cfg->dtype, [&](auto e) {
     using E = decltype(e);
-    k_head_norm_any<E><<<dim3((unsigned)tokens, (unsigned)heads), 64, 0, stream_of(stream)>>>(a);
+    const hipStream_t st = stream_of(stream);
+    // (halves that end inside a lane's 8 values take the general kernel)
+    const bool halves_fit = a.interleaved || a.R % 16 == 0;
+    if (d % 8 || d > kMaxFastDim || !halves_fit || !aligned16(a.s[0]) || (k && !aligned16(a.s[1]))) {
+      k_head_norm_any<E><<<dim3((unsigned)tokens, (unsigned)heads), 64, 0, st>>>(a);
+      return;
+    }
+    auto go = [&](auto lanes) {
+      constexpr int kLanes = decltype(lanes)::value, kAtOnce = kThreads / kLanes;
+      // heads of a workgroup: as many as leave enough workgroups
+      const int64_t passes = (heads + kAtOnce - 1) / kAtOnce;
+      int64_t groups = (kEnough + tokens - 1) / tokens;
+      groups = groups < passes ? groups : passes;
+      const int per_group = (int)((passes + groups - 1) / groups) * kAtOnce;
+      k_head_norm<E, kLanes><<<dim3((unsigned)tokens, (unsigned)((heads + per_group - 1) / per_group)), kThreads, 0, st>>>(
+          a, per_group);
+    };
+    if (d <= 64) go(std::integral_constant<int, 8>{});
+    else if (d <= 128) go(std::integral_constant<int, 16>{});
+    else if (d <= 256) go(std::integral_constant<int, 32>{});
+    else go(std::integral_constant<int, 64>{});
   });
   EXL3_LAUNCHED("k_head_norm");
   return EXL3_OK;

@@ -9,17 +9,20 @@ import torch
 
 from . import _lib
 from ._lib import DeltaConfig, DeltaRows, call
-from .heads import ST_DTYPE, require, require_device
-from .trellis import _ptr, _stream, _workspace
+from .heads import ST_DTYPE, require, require_device, stream_on
+from .trellis import _ptr, _workspace
 
 
 def _rows(t: torch.Tensor, what: str, dtype, shape, device) -> int:
-    """Token stride of (tokens, ...) rows whose tokens are contiguous blocks."""
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != device:
+    """Token stride of (tokens, heads[, size]) rows whose tokens are contiguous blocks."""
+    if t.dtype != dtype or t.shape != shape or t.device != device:
         raise ValueError(f"delta_rule: {what} must be a {dtype} tensor of shape {tuple(shape)} on {device}")
-    if shape[0] and not t[0].is_contiguous():
-        raise ValueError(f"delta_rule: a token's {what} must be contiguous")
-    return t.stride(0)
+    strides, size = t.stride(), 1
+    for i in range(len(shape) - 1, 0, -1):
+        if strides[i] != size and shape[i] > 1:
+            raise ValueError(f"delta_rule: a token's {what} must be contiguous")
+        size *= shape[i]
+    return strides[0]
 
 
 def _config(q, v, g, scale) -> DeltaConfig:
@@ -68,5 +71,5 @@ def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     if ws is None or ws.numel() < need:
         ws = _workspace(need, dev)
     call("exl3_delta_rule", C.byref(cfg), C.byref(x), T, _ptr(starts), n, state.data_ptr(), state.shape[0],
-         _ptr(slots), _ptr(dst), ws.data_ptr(), ws.numel(), _stream())
+         _ptr(slots), _ptr(dst), ws.data_ptr(), ws.numel(), stream_on(dev))
     return out

@@ -19,8 +19,16 @@ MODES = {"rms": NORM_RMS, "l2": NORM_L2}
 
 def require(t: torch.Tensor, what: str, dtype, shape, device) -> None:
     """t is a contiguous tensor of this dtype and shape on this device."""
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != device:
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.device != device:
         raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
+
+
+# the current stream's handle of a device, without a Stream object for each call
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+
+
+def stream_on(device) -> int:
+    return _raw_stream(device.index) if _raw_stream is not None else _stream()
 
 
 def require_device(t: torch.Tensor, what: str) -> None:
@@ -30,14 +38,14 @@ def require_device(t: torch.Tensor, what: str) -> None:
 
 
 def _side(what, x, w, y, dtype, device):
-    if x.dim() != 3 or x.dtype != dtype or x.device != device or (x.shape[2] > 1 and x.stride(2) != 1):
+    shape, xs, ys = x.shape, x.stride(), y.stride()
+    if len(shape) != 3 or x.dtype != dtype or x.device != device or (shape[2] > 1 and xs[2] != 1):
         raise ValueError(f"head_norm: {what} must be (tokens, heads, head_dim) with adjacent values, of one dtype and device")
-    if y.shape != x.shape or y.dtype != dtype or y.device != device or (y.shape[2] > 1 and y.stride(2) != 1):
+    if y.shape != shape or y.dtype != dtype or y.device != device or (shape[2] > 1 and ys[2] != 1):
         raise ValueError(f"head_norm: {what}'s output must have its shape, dtype and device")
     if w is not None:
-        require(w, f"head_norm: {what}'s weight", dtype, (x.shape[2],), device)
-    return HeadRows(x.data_ptr(), None if w is None else w.data_ptr(), y.data_ptr(), x.shape[1],
-                    x.stride(0), x.stride(1), y.stride(0), y.stride(1))
+        require(w, f"head_norm: {what}'s weight", dtype, (shape[2],), device)
+    return HeadRows(x.data_ptr(), None if w is None else w.data_ptr(), y.data_ptr(), shape[1], xs[0], xs[1], ys[0], ys[1])
 
 
 def head_norm(q: torch.Tensor, k: torch.Tensor | None = None, *, mode: str = "rms", eps: float = 1e-6,
@@ -65,13 +73,13 @@ def head_norm(q: torch.Tensor, k: torch.Tensor | None = None, *, mode: str = "rm
         rotate = 2 * inv_freq.numel()
         if rotate > d:
             raise ValueError("head_norm: inv_freq has more than head_dim / 2 frequencies")
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+    q_out = q.new_empty(q.shape) if q_out is None else q_out
     sides = [_side("q", q, q_weight, q_out, q.dtype, q.device)]
     if k is not None:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else k_out
+        k_out = k.new_empty(k.shape) if k_out is None else k_out
         sides.append(_side("k", k, k_weight, k_out, q.dtype, q.device))
     require_device(q, "head_norm")
     cfg = HeadNormConfig(ST_DTYPE[q.dtype], MODES[mode], d, rotate, int(interleaved), eps)
     call("exl3_head_norm", C.byref(cfg), C.byref(sides[0]), C.byref(sides[1]) if k is not None else None, T,
-         None if positions is None else positions.data_ptr(), None if inv_freq is None else inv_freq.data_ptr(), _stream())
+         None if positions is None else positions.data_ptr(), None if inv_freq is None else inv_freq.data_ptr(), stream_on(q.device))
     return q_out if k is None else (q_out, k_out)

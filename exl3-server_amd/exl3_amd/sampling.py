@@ -8,8 +8,8 @@ import torch
 
 from . import _lib
 from ._lib import SampleConfig, call
-from .heads import ST_DTYPE, require, require_device
-from .trellis import _stream, _workspace
+from .heads import ST_DTYPE, require, require_device, stream_on
+from .trellis import _workspace
 
 
 def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
@@ -48,5 +48,5 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     if ws is None or ws.numel() < need:
         ws = _workspace(need, dev)
     call("exl3_sample", C.byref(cfg), logits.data_ptr(), rows, vocab, max(vocab, logits.stride(0)), u.data_ptr(),
-         ids.data_ptr(), probs.data_ptr(), ws.data_ptr(), ws.numel(), _stream())
+         ids.data_ptr(), probs.data_ptr(), ws.data_ptr(), ws.numel(), stream_on(dev))
     return ids, probs
