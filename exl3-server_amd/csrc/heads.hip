@@ -37,8 +37,8 @@ struct HeadSide {
 struct HeadArgs {
   HeadSide s[2];
   int64_t tokens;
-  int32_t d, R, interleaved, l2;
-  float eps;
+  int32_t d, R, interleaved;
+  float mean, eps;  // mean: 1 / d, or 1 for the L2 norm
   const int32_t *positions;
   const float *inv_freq;
 };
@@ -52,7 +52,7 @@ __device__ __forceinline__ float2 turn(int32_t pos, float inv_freq) {
 }
 
 __device__ __forceinline__ float scale_of(const HeadArgs &a, float sq) {
-  return 1.0f / sqrtf((a.l2 ? sq : sq / (float)a.d) + a.eps);
+  return __builtin_amdgcn_rsqf(fmaf(sq, a.mean, a.eps));
 }
 
 // Any head size up to 1024, any strides: a wave per head, values one by one, the normed head
@@ -265,7 +265,7 @@ extern "C" exl3_status exl3_head_norm(const exl3_head_norm_config *cfg, const ex
   a.d = d;
   a.R = cfg->rotate_dims;
   a.interleaved = cfg->interleaved != 0;
-  a.l2 = cfg->mode == EXL3_NORM_L2;
+  a.mean = cfg->mode == EXL3_NORM_L2 ? 1.0f : 1.0f / (float)d;
   a.eps = cfg->eps;
   a.positions = positions;
   a.inv_freq = inv_freq;
