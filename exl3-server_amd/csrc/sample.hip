@@ -10,7 +10,8 @@
 // Every weight is taken in f64 and held as an integer of 2^-44 of the largest: sums of
 // integers are the same in any order, so the histogram's atomics and the split over
 // workgroups change nothing, and a row of 2^19 tokens fits 64 bits. (A weight under 2^-45 of
-// the largest counts as 0.)
+// the largest counts as 0.) Rows are read in 16-byte pieces, several in flight; a product in
+// f32 tells first which tokens can matter, and only those are weighed.
 //
 //  k_sample_max   grid (split, row): the split's largest logit and its index.
 //  k_sample_hist  grid (split, row): counts and weights of the split's tokens in bins of 1/64
@@ -22,6 +23,7 @@
 //                 (11, 11, 10) with the same histogram.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <string>
 
 #include "elem.hpp"
@@ -39,7 +41,7 @@ constexpr int kBins = 2048;           // 2000 used
 constexpr double kPerT = 64.0;        // bins per unit of t
 constexpr double kMaxT = 31.25;       // exp(-31.25) < 2^-45
 constexpr double kOne = 17592186044416.0;  // 2^44
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kPickThreads = 1024;
 constexpr int kList = 2048;           // tokens of a sorted list
 constexpr int kMaxSplits = 16;
@@ -81,21 +83,71 @@ __device__ __forceinline__ double temperature_of(const SampleArgs &a, int64_t ro
   return (double)(a.temperatures ? a.temperatures[row] : a.temperature);
 }
 
-// The weight of a token against the row's largest logit m: t, or a t past kMaxT where it has none.
+// A row's tokens against its largest logit m.
 struct Weigher {
-  float m;
-  double temp;
-  __device__ __forceinline__ double t(uint32_t key) const {
-    if (key <= kMaskedKey) return 1e300;
-    const float x = of_key(key);
+  float m, half_m, scale;  // scale: 2 / temperature
+  double inv;
+  __device__ __forceinline__ Weigher(float m, double temp)
+      : m(m), half_m(0.5f * m), scale((float)(2.0 / temp)), inv(1.0 / temp) {}
+  // Whether t may lie in [lo, hi]: halved so that no difference overflows; off by less than the
+  // margin of 1e-3 up to kMaxT. NaN (both infinite, or a temperature past f32) may.
+  __device__ __forceinline__ bool near(float x, float lo, float hi) const {
+    const float t = (half_m - 0.5f * x) * scale;
+    return !(t < lo - 1e-3f) && !(t > hi + 1e-3f);
+  }
+  // t, or one past kMaxT for a token that is never taken.
+  __device__ __forceinline__ double t(float x) const {
+    if (!(x > -INFINITY)) return 1e300;
     if (x == m) return 0.0;  // also +inf
-    const double d = ((double)m - (double)x) / temp;
+    const double d = ((double)m - (double)x) * inv;
     return d < 1e300 ? d : 1e300;
   }
   static __device__ __forceinline__ int bin(double t) { return (int)(t * kPerT); }
-  static __device__ __forceinline__ double w(double t) { return exp(-t); }
-  static __device__ __forceinline__ u64 fixed(double w) { return (u64)rint(w * kOne); }
+  // exp(-t) 2^44 for t <= kMaxT: -t = (n + f) ln 2, the series of e^(f ln 2) up to the 11th power
+  // (off by 7e-15 of itself).
+  static __device__ __forceinline__ double weight(double t) {
+    const double y = t * -1.4426950408889634074, n = rint(y), r = (y - n) * 0.69314718055994530942;
+    double p = 2.5052108385441719e-8;
+    p = fma(p, r, 2.7557319223985891e-7);
+    p = fma(p, r, 2.7557319223985893e-6);
+    p = fma(p, r, 2.4801587301587302e-5);
+    p = fma(p, r, 1.9841269841269841e-4);
+    p = fma(p, r, 1.3888888888888889e-3);
+    p = fma(p, r, 8.3333333333333333e-3);
+    p = fma(p, r, 4.1666666666666667e-2);
+    p = fma(p, r, 0.16666666666666667);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return ldexp(p, (int)n + 44);
+  }
+  // To the nearest integer: the sum's low bits are it.
+  static __device__ __forceinline__ u64 fixed(double w) {
+    return bitcast<u64>(w + 4503599627370496.0) & 0x000fffffffffffffull;
+  }
 };
+
+// f(index, value) for the values [first, last) of a row, by `step` threads of which this is
+// thread tid: 16-byte pieces, kAhead of them loaded before the first is taken; what is left
+// of a row one by one.
+template <typename E, int kAhead, typename F>
+__device__ __forceinline__ void each_value(const E *row, int first, int last, int tid, int step, F &&f) {
+  constexpr int N = 16 / sizeof(E);
+  typedef E piece __attribute__((ext_vector_type(N), aligned(sizeof(E))));
+  const int pieces = (last - first) / N;
+  for (int p = tid; p < pieces; p += kAhead * step) {
+    piece x[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      x[k] = *reinterpret_cast<const piece *>(row + first + (int64_t)min(p + k * step, pieces - 1) * N);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (p + k * step < pieces)
+#pragma unroll
+        for (int i = 0; i < N; ++i) f(first + (p + k * step) * N + i, to_f32((E)x[k][i]));
+  }
+  for (int i = first + pieces * N + tid; i < last; i += step) f(i, to_f32(row[i]));
+}
 
 template <typename T, typename Op>
 __device__ __forceinline__ T wave_reduce(T v, Op op) {
@@ -117,11 +169,14 @@ __global__ __launch_bounds__(kThreads) void k_sample_max(SampleArgs a) {
   const int64_t row = blockIdx.y;
   const int first = blockIdx.x * a.per_split, last = min(a.vocab, first + a.per_split);
   const E *x = reinterpret_cast<const E *>(a.logits) + row * a.stride;
-  u64 b = 0;
-  for (int i = first + threadIdx.x; i < last; i += kThreads) {
-    const u64 v = (u64)key_of(to_f32(x[i])) << 32 | (uint32_t)~i;
-    b = v > b ? v : b;
-  }
+  // (a thread's indices ascend, so the first of equal keys stays)
+  uint32_t most = 0;
+  int at = first;
+  each_value<E, 4>(x, first, last, threadIdx.x, kThreads, [&](int i, float v) {
+    const uint32_t k = key_of(v);
+    if (k > most) most = k, at = i;
+  });
+  u64 b = (u64)most << 32 | (uint32_t)~at;
   b = wave_reduce(b, [](u64 p, u64 q) { return p > q ? p : q; });
   if ((threadIdx.x & 63) == 0) red[threadIdx.x / 64] = b;
   __syncthreads();
@@ -142,21 +197,21 @@ __global__ __launch_bounds__(kThreads) void k_sample_hist(SampleArgs a) {
   if (!(temp > 0.0) || (uint32_t)(best >> 32) <= kMaskedKey) return;  // the first token, or none
   for (int i = threadIdx.x; i < kBins; i += kThreads) mass[i] = 0, count[i] = 0;
   __syncthreads();
-  const Weigher W{of_key((uint32_t)(best >> 32)), temp};
-  const double least = (double)(a.min_ps ? a.min_ps[row] : a.min_p);
+  const Weigher W(of_key((uint32_t)(best >> 32)), temp);
+  const double least = kOne * (double)(a.min_ps ? a.min_ps[row] : a.min_p);
   const int first = blockIdx.x * a.per_split, last = min(a.vocab, first + a.per_split);
   const E *x = reinterpret_cast<const E *>(a.logits) + row * a.stride;
   u64 above = 0;
-  for (int i = first + threadIdx.x; i < last; i += kThreads) {
-    const double t = W.t(key_of(to_f32(x[i])));
-    if (t < kMaxT) {
-      const double w = W.w(t);
-      const u64 f = W.fixed(w);
-      atomicAdd(&count[W.bin(t)], 1u);
-      atomicAdd(&mass[W.bin(t)], f);
-      if (!(w < least)) above += f;
-    }
-  }
+  each_value<E, 2>(x, first, last, threadIdx.x, kThreads, [&](int, float v) {
+    if (!W.near(v, 0.0f, (float)kMaxT)) return;
+    const double t = W.t(v);
+    if (t >= kMaxT) return;
+    const double w = W.weight(t);
+    const u64 f = W.fixed(w);
+    atomicAdd(&count[W.bin(t)], 1u);
+    atomicAdd(&mass[W.bin(t)], f);
+    if (!(w < least)) above += f;
+  });
   above = wave_reduce(above, [](u64 p, u64 q) { return p + q; });
   if ((threadIdx.x & 63) == 0) red[threadIdx.x / 64] = above;
   __syncthreads();
@@ -256,7 +311,16 @@ struct Row {
   const E *x;
   int vocab;
   Weigher W;
-  __device__ __forceinline__ uint32_t key(int i) const { return key_of(to_f32(x[i])); }
+  // f(index, value, t) for the tokens of bins [b0, b1]
+  template <typename F>
+  __device__ __forceinline__ void each_in(int b0, int b1, F &&f) const {
+    const float lo = b0 / (float)kPerT, hi = (b1 + 1) / (float)kPerT;
+    each_value<E, 4>(x, 0, vocab, threadIdx.x, kPickThreads, [&](int i, float v) {
+      if (!W.near(v, lo, hi)) return;
+      const double t = W.t(v);
+      if (t < kMaxT && W.bin(t) >= b0 && W.bin(t) <= b1) f(i, v, t);
+    });
+  }
 };
 
 // The first token of the sorted list where `u` is met, with `before` in front of the list (the
@@ -267,7 +331,7 @@ __device__ Found in_list(PickShared &s, const Row<E> &row, int n, const Until &u
   u64 own[2], m = 0;
   for (int k = 0; k < 2; ++k) {
     const int i = 2 * tid + k;
-    own[k] = i < n ? row.W.fixed(row.W.w(row.W.t((uint32_t)~(s.list[i] >> 32)))) : 0;
+    own[k] = i < n ? row.W.fixed(row.W.weight(row.W.t(of_key((uint32_t)~(s.list[i] >> 32))))) : 0;
     m += own[k];
   }
 #pragma unroll
@@ -300,17 +364,10 @@ template <typename E>
 __device__ int gather(PickShared &s, const Row<E> &row, int b0, int b1) {
   if (threadIdx.x == 0) s.n = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < row.vocab; i += kPickThreads) {
-    const uint32_t k = row.key(i);
-    const double t = row.W.t(k);
-    if (t < kMaxT) {
-      const int b = Weigher::bin(t);
-      if (b >= b0 && b <= b1) {
-        const int at = atomicAdd(&s.n, 1);
-        if (at < kList) s.list[at] = (u64)(uint32_t)~k << 32 | (uint32_t)i;
-      }
-    }
-  }
+  row.each_in(b0, b1, [&](int i, float v, double) {
+    const int at = atomicAdd(&s.n, 1);
+    if (at < kList) s.list[at] = (u64)(uint32_t)~key_of(v) << 32 | (uint32_t)i;
+  });
   __syncthreads();
   const int n = min(s.n, kList);
   sort_list(s, n);
@@ -329,16 +386,13 @@ __device__ Found in_bin(PickShared &s, const Row<E> &row, int bin, const Until &
     const int bits = round < 2 ? 11 : 10, next = low - bits;
     for (int i = tid; i < kBins; i += kPickThreads) s.mass[i] = 0, s.count[i] = 0;
     __syncthreads();
-    for (int i = tid; i < row.vocab; i += kPickThreads) {
-      const uint32_t k = row.key(i), c = ~k;
-      if (low < 32 && (c ^ prefix) >> low) continue;
-      const double t = row.W.t(k);
-      if (t < kMaxT && Weigher::bin(t) == bin) {
-        const int at = (c >> next) & ((1 << bits) - 1);
-        atomicAdd(&s.count[at], 1u);
-        atomicAdd(&s.mass[at], Weigher::fixed(Weigher::w(t)));
-      }
-    }
+    row.each_in(bin, bin, [&](int, float v, double t) {
+      const uint32_t c = ~key_of(v);
+      if (low < 32 && (c ^ prefix) >> low) return;
+      const int at = (c >> next) & ((1 << bits) - 1);
+      atomicAdd(&s.count[at], 1u);
+      atomicAdd(&s.mass[at], Weigher::fixed(Weigher::weight(t)));
+    });
     __syncthreads();
     scan_bins(s);
     const Until here{u.kind, u.kind == Until::kCount ? u.count - before_count : 0, u.mass};
@@ -359,11 +413,12 @@ __device__ Found in_bin(PickShared &s, const Row<E> &row, int bin, const Until &
   }
   // ties: how many of this logit it takes, and which index that is
   const uint32_t key = ~prefix;
-  const u64 w = Weigher::fixed(Weigher::w(row.W.t(key)));
+  const float logit = of_key(key);
+  const u64 w = Weigher::fixed(Weigher::weight(row.W.t(logit)));
   uint32_t ties = 0;
   {
     u64 c = 0;
-    for (int i = tid; i < row.vocab; i += kPickThreads) c += row.key(i) == key;
+    each_value<E, 4>(row.x, 0, row.vocab, tid, kPickThreads, [&](int, float v) { c += v == logit; });
     c = wave_reduce(c, [](u64 p, u64 q) { return p + q; });
     if ((tid & 63) == 0) s.wave_count[tid >> 6] = (uint32_t)c;
     __syncthreads();
@@ -381,7 +436,7 @@ __device__ Found in_bin(PickShared &s, const Row<E> &row, int bin, const Until &
   uint32_t seen = 0;
   for (int base = 0; base < row.vocab; base += kPickThreads) {
     const int i = base + tid;
-    const bool hit = i < row.vocab && row.key(i) == key;
+    const bool hit = i < row.vocab && to_f32(row.x[i]) == logit;
     const u64 votes = __ballot(hit);
     if ((tid & 63) == 0) s.wave_count[tid >> 6] = __popcll(votes);
     __syncthreads();
@@ -416,12 +471,13 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
     return;
   }
   const Row<E> row{reinterpret_cast<const E *>(a.logits) + r * a.stride, a.vocab,
-                   Weigher{of_key((uint32_t)(best >> 32)), temp}};
+                   Weigher(of_key((uint32_t)(best >> 32)), temp)};
   // bins of the whole row, added up from its splits and scanned
   auto whole_row = [&] {
     for (int i = tid; i < kBins; i += kPickThreads) {
       u64 m = 0;
       uint32_t c = 0;
+#pragma unroll 8
       for (int k = 0; k < a.splits; ++k) {
         m += a.mass[(r * a.splits + k) * kBins + i];
         c += a.count[(r * a.splits + k) * kBins + i];
@@ -462,7 +518,7 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
   if (top_p < 1.0f) kept = find(Until{Until::kAtLeast, 0, (double)top_p * (double)kept}).mass;
   u64 above = tid % 64 < a.splits ? a.min_mass[r * a.splits + tid % 64] : 0;
   above = wave_reduce(above, [](u64 p, u64 q) { return p + q; });
-  const u64 first = Weigher::fixed(1.0);
+  const u64 first = (u64)kOne;
   above = above < first ? first : above;
   kept = above < kept ? above : kept;
   const float u = a.u[r];
@@ -471,7 +527,7 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
   const Found f = goal < (double)kept ? find(Until{Until::kMore, 0, goal}) : find(Until{Until::kAtLeast, 0, (double)kept});
   if (tid == 0) {
     a.ids[r] = f.id;
-    if (a.probs) a.probs[r] = (float)(Weigher::w(row.W.t(f.key)) / ((double)kept / kOne));
+    if (a.probs) a.probs[r] = (float)(exp(-row.W.t(of_key(f.key))) / ((double)kept / kOne));
   }
 }
 
