@@ -25,6 +25,7 @@
 
 #include <cmath>
 #include <string>
+#include <type_traits>
 
 #include "elem.hpp"
 #include "exl3_device.hpp"
@@ -85,15 +86,18 @@ __device__ __forceinline__ double temperature_of(const SampleArgs &a, int64_t ro
 
 // A row's tokens against its largest logit m.
 struct Weigher {
-  float m, half_m, scale;  // scale: 2 / temperature
-  double inv;
-  __device__ __forceinline__ Weigher(float m, double temp)
-      : m(m), half_m(0.5f * m), scale((float)(2.0 / temp)), inv(1.0 / temp) {}
-  // Whether t may lie in [lo, hi]: halved so that no difference overflows; off by less than the
-  // margin of 1e-3 up to kMaxT. NaN (both infinite, or a temperature past f32) may.
-  __device__ __forceinline__ bool near(float x, float lo, float hi) const {
-    const float t = (half_m - 0.5f * x) * scale;
-    return !(t < lo - 1e-3f) && !(t > hi + 1e-3f);
+  float m;
+  double temp, inv;
+  __device__ __forceinline__ Weigher(float m, double temp) : m(m), temp(temp), inv(1.0 / temp) {}
+  // The logits whose t may lie in [lo, hi], with a margin for the roundings of its ends.
+  struct Range {
+    float least, most;
+    __device__ __forceinline__ bool has(float x) const { return x >= least && x <= most; }
+  };
+  __device__ __forceinline__ Range range(double lo, double hi) const {
+    if (m == INFINITY) return Range{m, m};
+    const double least = (double)m - temp * (hi + 1e-3), most = (double)m - temp * (lo - 1e-3);
+    return Range{(float)(least - 1e-6 * fabs(least) - 1e-40), (float)(most + 1e-6 * fabs(most) + 1e-40)};
   }
   // t, or one past kMaxT for a token that is never taken.
   __device__ __forceinline__ double t(float x) const {
@@ -127,11 +131,16 @@ struct Weigher {
   }
 };
 
-// f(index, value) for the values [first, last) of a row, by `step` threads of which this is
-// thread tid: 16-byte pieces, kAhead of them loaded before the first is taken; what is left
-// of a row one by one.
-template <typename E, int kAhead, typename F>
-__device__ __forceinline__ void each_value(const E *row, int first, int last, int tid, int step, F &&f) {
+struct AllValues {
+  __device__ __forceinline__ bool has(float) const { return true; }
+};
+
+// f(index, value) for the values [first, last) of a row that `wanted` has, by `step` threads of
+// which this is thread tid: 16-byte pieces, kAhead of them loaded before the first is taken;
+// what is left of a row one by one. Pieces with no wanted value in a whole wave cost
+// their comparisons alone.
+template <typename E, int kAhead, typename R, typename F>
+__device__ __forceinline__ void each_value(const E *row, int first, int last, int tid, int step, const R &wanted, F &&f) {
   constexpr int N = 16 / sizeof(E);
   typedef E piece __attribute__((ext_vector_type(N), aligned(sizeof(E))));
   const int pieces = (last - first) / N;
@@ -141,12 +150,31 @@ __device__ __forceinline__ void each_value(const E *row, int first, int last, in
     for (int k = 0; k < kAhead; ++k)
       x[k] = *reinterpret_cast<const piece *>(row + first + (int64_t)min(p + k * step, pieces - 1) * N);
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if (p + k * step < pieces)
+    for (int k = 0; k < kAhead; ++k) {
+      uint32_t which = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) which |= wanted.has(to_f32((E)x[k][i])) ? 1u << i : 0u;
+      if (p + k * step >= pieces) which = 0;
+      if constexpr (!std::is_same_v<R, AllValues>) {
+        // few are wanted: one at a time
+        while (which) {
+          const int i = __ffs(which) - 1;
+          which &= which - 1;
+          float v = 0.0f;
+#pragma unroll
+          for (int n = 0; n < N; ++n) v = n == i ? to_f32((E)x[k][n]) : v;
+          f(first + (p + k * step) * N + i, v);
+        }
+      } else if (which) {
 #pragma unroll
         for (int i = 0; i < N; ++i) f(first + (p + k * step) * N + i, to_f32((E)x[k][i]));
+      }
+    }
   }
-  for (int i = first + pieces * N + tid; i < last; i += step) f(i, to_f32(row[i]));
+  for (int i = first + pieces * N + tid; i < last; i += step) {
+    const float v = to_f32(row[i]);
+    if (wanted.has(v)) f(i, v);
+  }
 }
 
 template <typename T, typename Op>
@@ -172,7 +200,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_max(SampleArgs a) {
   // (a thread's indices ascend, so the first of equal keys stays)
   uint32_t most = 0;
   int at = first;
-  each_value<E, 4>(x, first, last, threadIdx.x, kThreads, [&](int i, float v) {
+  each_value<E, 4>(x, first, last, threadIdx.x, kThreads, AllValues{}, [&](int i, float v) {
     const uint32_t k = key_of(v);
     if (k > most) most = k, at = i;
   });
@@ -202,8 +230,9 @@ __global__ __launch_bounds__(kThreads) void k_sample_hist(SampleArgs a) {
   const int first = blockIdx.x * a.per_split, last = min(a.vocab, first + a.per_split);
   const E *x = reinterpret_cast<const E *>(a.logits) + row * a.stride;
   u64 above = 0;
-  each_value<E, 2>(x, first, last, threadIdx.x, kThreads, [&](int, float v) {
-    if (!W.near(v, 0.0f, (float)kMaxT)) return;
+  const Weigher::Range weighed = W.range(0.0, kMaxT);
+  each_value<E, 2>(x, first, last, threadIdx.x, kThreads, AllValues{}, [&](int, float v) {
+    if (!weighed.has(v)) return;
     const double t = W.t(v);
     if (t >= kMaxT) return;
     const double w = W.weight(t);
@@ -314,9 +343,7 @@ struct Row {
   // f(index, value, t) for the tokens of bins [b0, b1]
   template <typename F>
   __device__ __forceinline__ void each_in(int b0, int b1, F &&f) const {
-    const float lo = b0 / (float)kPerT, hi = (b1 + 1) / (float)kPerT;
-    each_value<E, 4>(x, 0, vocab, threadIdx.x, kPickThreads, [&](int i, float v) {
-      if (!W.near(v, lo, hi)) return;
+    each_value<E, 4>(x, 0, vocab, threadIdx.x, kPickThreads, W.range(b0 / kPerT, (b1 + 1) / kPerT), [&](int i, float v) {
       const double t = W.t(v);
       if (t < kMaxT && W.bin(t) >= b0 && W.bin(t) <= b1) f(i, v, t);
     });
@@ -418,7 +445,7 @@ __device__ Found in_bin(PickShared &s, const Row<E> &row, int bin, const Until &
   uint32_t ties = 0;
   {
     u64 c = 0;
-    each_value<E, 4>(row.x, 0, row.vocab, tid, kPickThreads, [&](int, float v) { c += v == logit; });
+    each_value<E, 4>(row.x, 0, row.vocab, tid, kPickThreads, AllValues{}, [&](int, float v) { c += v == logit; });
     c = wave_reduce(c, [](u64 p, u64 q) { return p + q; });
     if ((tid & 63) == 0) s.wave_count[tid >> 6] = (uint32_t)c;
     __syncthreads();
