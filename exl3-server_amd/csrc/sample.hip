@@ -15,12 +15,13 @@
 //
 //  k_sample_max   grid (split, row): the split's largest logit and its index.
 //  k_sample_hist  grid (split, row): counts and weights of the split's tokens in bins of 1/64
-//                 of t (2000 bins down to 2^-45), and the count and weight at min_p or above.
-//  k_sample_pick  a workgroup per row: the splits' histograms added up and scanned give the
-//                 bins in which top-k, top-p and the random number end; only those bins'
-//                 tokens are gathered from the row, sorted and summed token by token. A bin
-//                 with more tokens than the list holds is narrowed by the logits' bits
-//                 (11, 11, 10) with the same histogram.
+//                 of t (2000 bins down to 2^-45) and in groups of 32 bins, the tokens' indices
+//                 in the bins' order, and the weight at min_p or above.
+//  k_sample_pick  a workgroup per row, for each end of a beginning (top-k, top-p, the random
+//                 number): the group it falls in, the bin of the group, the bin's tokens by way
+//                 of the splits' index lists, and their order; only those tokens' logits are
+//                 read again. A bin with more tokens than the list holds is narrowed by their
+//                 logits' and indices' bits, 11 at a time.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -43,12 +44,13 @@ constexpr double kPerT = 64.0;        // bins per unit of t
 constexpr double kMaxT = 31.25;       // exp(-31.25) < 2^-45
 constexpr double kOne = 17592186044416.0;  // 2^44
 constexpr int kThreads = 512;
-constexpr int kPickThreads = 1024;
-constexpr int kList = 2048;           // tokens of a sorted list
-constexpr int kMaxSplits = 16;
-static_assert(kMaxSplits <= 64, "a lane per split");
+constexpr int kGroups = 64, kInGroup = kBins / kGroups;
+constexpr int kList = 1024;           // tokens ordered at once
+constexpr int kMaxSplits = 64, kPerSplit = 8192;  // a lane per split; 13-bit places
+constexpr int kNoBin = 0xffff;
 static_assert(kMaxT * kPerT < kBins, "every weighted token has a bin");
-static_assert(kList == kBins && kPickThreads * 2 == kBins, "two bins a thread");
+static_assert(kMaxSplits * kPerSplit >= kMaxVocab, "the splits hold any row");
+static_assert(kThreads * 4 == kBins && kInGroup == 32, "four bins a thread, eight threads a group");
 
 typedef unsigned long long u64;
 
@@ -74,10 +76,14 @@ struct SampleArgs {
   const float *u;
   int32_t *ids;
   float *probs;
-  u64 *best;        // (rows, splits): key << 32 | ~index of the split's first token
-  u64 *mass;        // (rows, splits, kBins)
-  uint32_t *count;  // (rows, splits, kBins)
-  u64 *min_mass;    // (rows, splits): weight at min_p or above
+  // for each row and split
+  u64 *best;            // key << 32 | ~index of the first token
+  u64 *min_mass;        // weight at min_p or above
+  u64 *mass;            // (kBins)
+  uint32_t *place;      // (kBins): where a bin's indices begin, << 16 | their count
+  u64 *group_mass;      // (kGroups)
+  uint32_t *group_count;
+  uint16_t *order;      // (per_split): indices in the split, by bin
 };
 
 __device__ __forceinline__ double temperature_of(const SampleArgs &a, int64_t row) {
@@ -86,18 +92,16 @@ __device__ __forceinline__ double temperature_of(const SampleArgs &a, int64_t ro
 
 // A row's tokens against its largest logit m.
 struct Weigher {
-  float m;
-  double temp, inv;
-  __device__ __forceinline__ Weigher(float m, double temp) : m(m), temp(temp), inv(1.0 / temp) {}
-  // The logits whose t may lie in [lo, hi], with a margin for the roundings of its ends.
-  struct Range {
-    float least, most;
-    __device__ __forceinline__ bool has(float x) const { return x >= least && x <= most; }
-  };
-  __device__ __forceinline__ Range range(double lo, double hi) const {
-    if (m == INFINITY) return Range{m, m};
-    const double least = (double)m - temp * (hi + 1e-3), most = (double)m - temp * (lo - 1e-3);
-    return Range{(float)(least - 1e-6 * fabs(least) - 1e-40), (float)(most + 1e-6 * fabs(most) + 1e-40)};
+  float m, half_m, per;  // per: bins per half a logit
+  double inv;
+  __device__ __forceinline__ Weigher(float m, double temp)
+      : m(m), half_m(0.5f * m), per((float)(2.0 * kPerT / temp)), inv(1.0 / temp) {}
+  // The token's bin, by f32 alone (it only has to ascend as the logit falls; halved so that no
+  // difference overflows); kNoBin past the last one and for tokens that are never taken.
+  __device__ __forceinline__ int bin(float x) const {
+    if (x == m) return x > -INFINITY ? 0 : kNoBin;  // also +inf
+    const float b = (half_m - 0.5f * x) * per;
+    return b < (float)(kMaxT * kPerT) ? (int)b : kNoBin;  // (no for NaN)
   }
   // t, or one past kMaxT for a token that is never taken.
   __device__ __forceinline__ double t(float x) const {
@@ -106,10 +110,10 @@ struct Weigher {
     const double d = ((double)m - (double)x) * inv;
     return d < 1e300 ? d : 1e300;
   }
-  static __device__ __forceinline__ int bin(double t) { return (int)(t * kPerT); }
-  // exp(-t) 2^44 for t <= kMaxT: -t = (n + f) ln 2, the series of e^(f ln 2) up to the 11th power
+  // exp(-t) 2^44 (0 from 40 on): -t = (n + f) ln 2, the series of e^(f ln 2) up to the 11th power
   // (off by 7e-15 of itself).
   static __device__ __forceinline__ double weight(double t) {
+    if (t > 40.0) return 0.0;
     const double y = t * -1.4426950408889634074, n = rint(y), r = (y - n) * 0.69314718055994530942;
     double p = 2.5052108385441719e-8;
     p = fma(p, r, 2.7557319223985891e-7);
@@ -131,16 +135,11 @@ struct Weigher {
   }
 };
 
-struct AllValues {
-  __device__ __forceinline__ bool has(float) const { return true; }
-};
-
-// f(index, value) for the values [first, last) of a row that `wanted` has, by `step` threads of
-// which this is thread tid: 16-byte pieces, kAhead of them loaded before the first is taken;
-// what is left of a row one by one. Pieces with no wanted value in a whole wave cost
-// their comparisons alone.
-template <typename E, int kAhead, typename R, typename F>
-__device__ __forceinline__ void each_value(const E *row, int first, int last, int tid, int step, const R &wanted, F &&f) {
+// f(index, value) for the values [first, last) of a row, by `step` threads of which this is
+// thread tid: 16-byte pieces, kAhead of them loaded before the first is taken; what is left
+// of a row one by one. A thread's indices ascend.
+template <typename E, int kAhead, typename F>
+__device__ __forceinline__ void each_value(const E *row, int first, int last, int tid, int step, F &&f) {
   constexpr int N = 16 / sizeof(E);
   typedef E piece __attribute__((ext_vector_type(N), aligned(sizeof(E))));
   const int pieces = (last - first) / N;
@@ -150,31 +149,12 @@ __device__ __forceinline__ void each_value(const E *row, int first, int last, in
     for (int k = 0; k < kAhead; ++k)
       x[k] = *reinterpret_cast<const piece *>(row + first + (int64_t)min(p + k * step, pieces - 1) * N);
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      uint32_t which = 0;
-#pragma unroll
-      for (int i = 0; i < N; ++i) which |= wanted.has(to_f32((E)x[k][i])) ? 1u << i : 0u;
-      if (p + k * step >= pieces) which = 0;
-      if constexpr (!std::is_same_v<R, AllValues>) {
-        // few are wanted: one at a time
-        while (which) {
-          const int i = __ffs(which) - 1;
-          which &= which - 1;
-          float v = 0.0f;
-#pragma unroll
-          for (int n = 0; n < N; ++n) v = n == i ? to_f32((E)x[k][n]) : v;
-          f(first + (p + k * step) * N + i, v);
-        }
-      } else if (which) {
+    for (int k = 0; k < kAhead; ++k)
+      if (p + k * step < pieces)
 #pragma unroll
         for (int i = 0; i < N; ++i) f(first + (p + k * step) * N + i, to_f32((E)x[k][i]));
-      }
-    }
   }
-  for (int i = first + pieces * N + tid; i < last; i += step) {
-    const float v = to_f32(row[i]);
-    if (wanted.has(v)) f(i, v);
-  }
+  for (int i = first + pieces * N + tid; i < last; i += step) f(i, to_f32(row[i]));
 }
 
 template <typename T, typename Op>
@@ -195,12 +175,12 @@ template <typename E>
 __global__ __launch_bounds__(kThreads) void k_sample_max(SampleArgs a) {
   __shared__ u64 red[kThreads / 64];
   const int64_t row = blockIdx.y;
-  const int first = blockIdx.x * a.per_split, last = min(a.vocab, first + a.per_split);
+  const int first = min(a.vocab, (int)blockIdx.x * a.per_split), last = min(a.vocab, first + a.per_split);
   const E *x = reinterpret_cast<const E *>(a.logits) + row * a.stride;
-  // (a thread's indices ascend, so the first of equal keys stays)
+  // (the first of equal keys stays)
   uint32_t most = 0;
   int at = first;
-  each_value<E, 4>(x, first, last, threadIdx.x, kThreads, AllValues{}, [&](int i, float v) {
+  each_value<E, 4>(x, first, last, threadIdx.x, kThreads, [&](int i, float v) {
     const uint32_t k = key_of(v);
     if (k > most) most = k, at = i;
   });
@@ -219,74 +199,86 @@ __global__ __launch_bounds__(kThreads) void k_sample_hist(SampleArgs a) {
   __shared__ u64 mass[kBins];
   __shared__ uint32_t count[kBins];
   __shared__ u64 red[kThreads / 64];
+  __shared__ uint32_t wave_count[kThreads / 64];
+  extern __shared__ __align__(16) uint16_t of_split[];  // per_split bins, then as many indices
   const int64_t row = blockIdx.y;
   const double temp = temperature_of(a, row);
   const u64 best = row_best(a, row);
   if (!(temp > 0.0) || (uint32_t)(best >> 32) <= kMaskedKey) return;  // the first token, or none
-  for (int i = threadIdx.x; i < kBins; i += kThreads) mass[i] = 0, count[i] = 0;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int i = tid; i < kBins; i += kThreads) mass[i] = 0, count[i] = 0;
   __syncthreads();
   const Weigher W(of_key((uint32_t)(best >> 32)), temp);
   const double least = kOne * (double)(a.min_ps ? a.min_ps[row] : a.min_p);
-  const int first = blockIdx.x * a.per_split, last = min(a.vocab, first + a.per_split);
+  const int first = min(a.vocab, (int)blockIdx.x * a.per_split), last = min(a.vocab, first + a.per_split);
   const E *x = reinterpret_cast<const E *>(a.logits) + row * a.stride;
   u64 above = 0;
-  const Weigher::Range weighed = W.range(0.0, kMaxT);
-  each_value<E, 2>(x, first, last, threadIdx.x, kThreads, AllValues{}, [&](int, float v) {
-    if (!weighed.has(v)) return;
-    const double t = W.t(v);
-    if (t >= kMaxT) return;
-    const double w = W.weight(t);
+  each_value<E, 2>(x, first, last, tid, kThreads, [&](int i, float v) {
+    const int b = W.bin(v);
+    of_split[i - first] = (uint16_t)b;
+    if (b == kNoBin) return;
+    const double w = W.weight(W.t(v));
     const u64 f = W.fixed(w);
-    atomicAdd(&count[W.bin(t)], 1u);
-    atomicAdd(&mass[W.bin(t)], f);
+    atomicAdd(&count[b], 1u);
+    atomicAdd(&mass[b], f);
     if (!(w < least)) above += f;
   });
   above = wave_reduce(above, [](u64 p, u64 q) { return p + q; });
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x / 64] = above;
+  if (lane == 0) red[wave] = above;
   __syncthreads();
-  const int64_t at = (row * a.splits + blockIdx.x) * kBins;
-  for (int i = threadIdx.x; i < kBins; i += kThreads) {
-    a.mass[at + i] = mass[i];
-    a.count[at + i] = count[i];
+  // this thread's four bins, and where they begin among the split's tokens
+  uint32_t c[4], upto = 0;
+  u64 m[4], sum = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    c[k] = count[4 * tid + k];
+    m[k] = mass[4 * tid + k];
+    upto += c[k];
+    sum += m[k];
   }
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < kThreads / 64; ++i) above += red[i];
-    a.min_mass[row * a.splits + blockIdx.x] = above;
-  }
-}
-
-// Running sums over two bins a thread: the bins' own values in, the sums up to and with them out.
-struct PickShared {
-  u64 mass[kBins];
-  u64 list[kList];  // ~key << 32 | index, ascending: the order
-  uint32_t count[kBins];
-  u64 wave_mass[kPickThreads / 64];
-  uint32_t wave_count[kPickThreads / 64];
-  int found, n;
-  u64 before_mass;
-  uint32_t before_count;
-};
-
-__device__ void scan_bins(PickShared &s) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const u64 m0 = s.mass[2 * tid], m1 = s.mass[2 * tid + 1];
-  const uint32_t c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
-  u64 m = m0 + m1;
-  uint32_t c = c0 + c1;
+  const uint32_t own = upto;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const u64 pm = __shfl_up(m, o);
-    const uint32_t pc = __shfl_up(c, o);
-    if (lane >= o) m += pm, c += pc;
+    const uint32_t v = __shfl_up(upto, o);
+    if (lane >= o) upto += v;
   }
-  if (lane == 63) s.wave_mass[wave] = m, s.wave_count[wave] = c;
+  if (lane == 63) wave_count[wave] = upto;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) m += s.wave_mass[w], c += s.wave_count[w];
-  s.mass[2 * tid + 1] = m;
-  s.mass[2 * tid] = m - m1;
-  s.count[2 * tid + 1] = c;
-  s.count[2 * tid] = c - c1;
+  for (int w = 0; w < wave; ++w) upto += wave_count[w];
+  const int64_t split = row * a.splits + blockIdx.x;
+  uint32_t begin = upto - own, group = own;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    a.mass[split * kBins + 4 * tid + k] = m[k];
+    a.place[split * kBins + 4 * tid + k] = begin << 16 | c[k];
+    count[4 * tid + k] = begin;
+    begin += c[k];
+  }
+#pragma unroll
+  for (int o = 1; o < kInGroup / 4; o <<= 1) {
+    sum += __shfl_xor(sum, o);
+    group += __shfl_xor(group, o);
+  }
+  if (tid % (kInGroup / 4) == 0) {
+    a.group_mass[split * kGroups + tid / (kInGroup / 4)] = sum;
+    a.group_count[split * kGroups + tid / (kInGroup / 4)] = group;
+  }
+  if (tid == 0) {
+    for (int i = 1; i < kThreads / 64; ++i) above += red[i];
+    a.min_mass[split] = above;
+  }
   __syncthreads();
+  // the indices in the bins' order (within a bin in any)
+  uint16_t *ordered = of_split + a.per_split;
+  for (int i = tid; i < last - first; i += kThreads) {
+    const int b = of_split[i];
+    if (b != kNoBin) ordered[atomicAdd(&count[b], 1u)] = (uint16_t)i;
+  }
+  __syncthreads();
+  uint32_t all = 0;
+  for (int w = 0; w < kThreads / 64; ++w) all += wave_count[w];
+  uint32_t *to = reinterpret_cast<uint32_t *>(a.order + split * a.per_split);
+  for (uint32_t i = tid; 2 * i < all; i += kThreads) to[i] = reinterpret_cast<const uint32_t *>(ordered)[i];
 }
 
 // What ends a beginning of the order: the first token at which `count` tokens are reached, or
@@ -300,190 +292,221 @@ struct Until {
   }
 };
 
-// The first of the scanned bins (descending weight) where `u` is met; kBins if none.
-__device__ int first_bin(PickShared &s, const Until &u) {
-  if (threadIdx.x == 0) s.found = kBins;
-  __syncthreads();
-  for (int i = threadIdx.x; i < kBins; i += kPickThreads)
-    if (u.met(s.count[i], s.mass[i]) && (i == 0 || !u.met(s.count[i - 1], s.mass[i - 1]))) s.found = i;
-  __syncthreads();
-  const int b = s.found;
-  __syncthreads();
-  return b;
-}
-
-// Sorts s.list[0..n) ascending; n <= kList.
-__device__ void sort_list(PickShared &s, int n) {
-  int size = 2;
-  while (size < n) size <<= 1;
-  for (int i = n + threadIdx.x; i < size; i += kPickThreads) s.list[i] = ~0ull;
-  __syncthreads();
-  for (int k = 2; k <= size; k <<= 1)
-    for (int j = k >> 1; j; j >>= 1) {
-      for (int i = threadIdx.x; i < size / 2; i += kPickThreads) {
-        const int p = 2 * i - (i & (j - 1)), q = p + j;
-        const u64 x = s.list[p], y = s.list[q];
-        if ((x > y) == ((p & k) == 0)) s.list[p] = y, s.list[q] = x;
-      }
-      __syncthreads();
-    }
-}
+// A token's place in the order as a number: ~key (32 bits), index (22 bits).
+__device__ __forceinline__ u64 rank_of(uint32_t key, int index) { return (u64)(uint32_t)~key << 22 | (uint32_t)index; }
+__device__ __forceinline__ uint32_t rank_key(u64 r) { return (uint32_t)~(r >> 22); }
+__device__ __forceinline__ int rank_index(u64 r) { return (int)(r & 0x3fffff); }
 
 struct Found {
-  int32_t id;
-  uint32_t key, count;  // its logit, and tokens and weight up to and with it
-  u64 mass;
+  u64 rank, mass;  // the token, and the weight up to and with it
 };
 
-template <typename E>
-struct Row {
-  const E *x;
-  int vocab;
-  Weigher W;
-  // f(index, value, t) for the tokens of bins [b0, b1]
-  template <typename F>
-  __device__ __forceinline__ void each_in(int b0, int b1, F &&f) const {
-    each_value<E, 4>(x, 0, vocab, threadIdx.x, kPickThreads, W.range(b0 / kPerT, (b1 + 1) / kPerT), [&](int i, float v) {
-      const double t = W.t(v);
-      if (t < kMaxT && W.bin(t) >= b0 && W.bin(t) <= b1) f(i, v, t);
-    });
-  }
+struct Item {
+  u64 rank, mass;
 };
 
-// The first token of the sorted list where `u` is met, with `before` in front of the list (the
-// last one where rounding leaves none). Every thread gets it.
-template <typename E>
-__device__ Found in_list(PickShared &s, const Row<E> &row, int n, const Until &u, uint32_t before_count, u64 before_mass) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  u64 own[2], m = 0;
-  for (int k = 0; k < 2; ++k) {
-    const int i = 2 * tid + k;
-    own[k] = i < n ? row.W.fixed(row.W.weight(row.W.t(of_key((uint32_t)~(s.list[i] >> 32))))) : 0;
-    m += own[k];
-  }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
+struct PickShared {
+  Item list[kList];
+  u64 mass[kBins];       // of the buckets of a bin too large for the list
+  uint32_t count[kBins];
+  uint32_t place[kMaxSplits][kInGroup];
+  u64 group_mass[kGroups], bin_mass[kInGroup];
+  uint32_t group_count[kGroups], bin_count[kInGroup];
+  uint32_t upto[kMaxSplits], begin[kMaxSplits];  // of the bin's tokens, by split
+  u64 wave_mass[kThreads / 64];
+  uint32_t wave_count[kThreads / 64];
+  Found found;
+  uint32_t bucket;
+};
+
+// Inclusive sums over a wave's first `n` lanes.
+__device__ __forceinline__ void wave_scan(int n, uint32_t &c, u64 &m) {
+  const int lane = threadIdx.x & 63;
+  for (int o = 1; o < n; o <<= 1) {
+    const uint32_t pc = __shfl_up(c, o);
     const u64 pm = __shfl_up(m, o);
-    if (lane >= o) m += pm;
+    if (lane >= o) c += pc, m += pm;
   }
-  if (lane == 63) s.wave_mass[wave] = m;
-  if (tid == 0) s.found = n - 1;
-  __syncthreads();
-  m += before_mass;
-  for (int w = 0; w < wave; ++w) m += s.wave_mass[w];
-  const u64 upto[2] = {m - own[1], m};
-  for (int k = 0; k < 2; ++k) {
-    const int i = 2 * tid + k;
-    if (i < n && u.met(before_count + i + 1, upto[k]) && (!u.met(before_count + i, upto[k] - own[k]) || i == 0))
-      atomicMin(&s.found, i);
-  }
-  __syncthreads();
-  const int at = s.found;
-  if (at / 2 == tid) s.before_mass = upto[at & 1];
-  __syncthreads();
-  const Found f{(int32_t)(uint32_t)s.list[at], (uint32_t)~(s.list[at] >> 32), before_count + at + 1, s.before_mass};
-  __syncthreads();
-  return f;
 }
 
-// The tokens of bins [b0, b1] into the list, sorted; there are at most kList.
 template <typename E>
-__device__ int gather(PickShared &s, const Row<E> &row, int b0, int b1) {
-  if (threadIdx.x == 0) s.n = 0;
-  __syncthreads();
-  row.each_in(b0, b1, [&](int i, float v, double) {
-    const int at = atomicAdd(&s.n, 1);
-    if (at < kList) s.list[at] = (u64)(uint32_t)~key_of(v) << 32 | (uint32_t)i;
-  });
-  __syncthreads();
-  const int n = min(s.n, kList);
-  sort_list(s, n);
-  return n;
-}
+struct Pick {
+  const SampleArgs &a;
+  PickShared &s;
+  const int64_t row;
+  const E *x;
+  const Weigher W;
+  uint32_t upto_count;  // this lane's group: tokens and weight up to and with it
+  u64 upto_mass;
 
-// As in_list, over the tokens of one bin of any size: the logits' bits from the top, 11, 11
-// and 10 of them, until all tokens left have one logit; of those the index decides. Uses
-// s.mass and s.count.
-template <typename E>
-__device__ Found in_bin(PickShared &s, const Row<E> &row, int bin, const Until &u, uint32_t before_count, u64 before_mass) {
-  const int tid = threadIdx.x;
-  uint32_t prefix = 0;  // the bits of ~key found so far, in place
-  int low = 32;         // bits below them
-  for (int round = 0; round < 3; ++round) {
-    const int bits = round < 2 ? 11 : 10, next = low - bits;
-    for (int i = tid; i < kBins; i += kPickThreads) s.mass[i] = 0, s.count[i] = 0;
+  __device__ Pick(const SampleArgs &a, PickShared &s, int64_t row, const Weigher &W)
+      : a(a), s(s), row(row), x(reinterpret_cast<const E *>(a.logits) + row * a.stride), W(W) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    if (tid < kGroups) s.group_mass[tid] = 0, s.group_count[tid] = 0;
     __syncthreads();
-    row.each_in(bin, bin, [&](int, float v, double t) {
-      const uint32_t c = ~key_of(v);
-      if (low < 32 && (c ^ prefix) >> low) return;
-      const int at = (c >> next) & ((1 << bits) - 1);
-      atomicAdd(&s.count[at], 1u);
-      atomicAdd(&s.mass[at], Weigher::fixed(Weigher::weight(t)));
-    });
+    u64 m = 0;
+    uint32_t c = 0;
+#pragma unroll 8
+    for (int k = tid >> 6; k < a.splits; k += kThreads / 64) {
+      m += a.group_mass[(row * a.splits + k) * kGroups + lane];
+      c += a.group_count[(row * a.splits + k) * kGroups + lane];
+    }
+    atomicAdd(&s.group_mass[lane], m);
+    atomicAdd(&s.group_count[lane], c);
     __syncthreads();
-    scan_bins(s);
-    const Until here{u.kind, u.kind == Until::kCount ? u.count - before_count : 0, u.mass};
-    if (tid == 0) s.found = kBins;
+    upto_mass = s.group_mass[lane];
+    upto_count = s.group_count[lane];
+    wave_scan(kGroups, upto_count, upto_mass);
+  }
+  __device__ __forceinline__ uint32_t tokens() const { return __shfl(upto_count, 63); }
+  __device__ __forceinline__ u64 weight() const { return __shfl(upto_mass, 63); }
+
+  // The j-th of the bin's tokens (by split, in a split in any order).
+  __device__ __forceinline__ int token(uint32_t j) const {
+    int k = 0;
+#pragma unroll
+    for (int o = kMaxSplits / 2; o; o >>= 1)
+      if (s.upto[k + o - 1] <= j) k += o;
+    const uint32_t at = s.begin[k] + j - (k ? s.upto[k - 1] : 0u);
+    return k * a.per_split + a.order[(row * a.splits + k) * a.per_split + at];
+  }
+  __device__ __forceinline__ u64 mass_of(float v) const { return W.fixed(W.weight(W.t(v))); }
+
+  // The first token of the order where `u` is met, or the last of all where none is. Called
+  // by the whole workgroup, and the same for all of it.
+  __device__ Found find(const Until &u) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    // its group of bins
+    u64 votes = __ballot(u.met(upto_count, upto_mass));
+    if (!votes) votes = __ballot(upto_count == tokens());
+    const int g = __ffsll(votes) - 1;
+    uint32_t before_count = g ? __shfl(upto_count, g - 1) : 0;
+    u64 before_mass = g ? __shfl(upto_mass, g - 1) : 0;
+    // its bin
     __syncthreads();
-    const uint32_t all = s.count[kBins - 1];
-    for (int i = tid; i < kBins; i += kPickThreads) {
-      const uint32_t c0 = i ? s.count[i - 1] : 0;
-      if (s.count[i] > c0 && (here.met(s.count[i], before_mass + s.mass[i]) || s.count[i] == all)) atomicMin(&s.found, i);
+    if (tid < kInGroup) s.bin_mass[tid] = 0, s.bin_count[tid] = 0;
+    __syncthreads();
+    {
+      const int b = tid % kInGroup;
+      u64 m = 0;
+      uint32_t c = 0;
+#pragma unroll 4
+      for (int k = tid / kInGroup; k < a.splits; k += kThreads / kInGroup) {
+        const int64_t at = (row * a.splits + k) * kBins + g * kInGroup + b;
+        const uint32_t place = a.place[at];
+        m += a.mass[at];
+        c += place & 0xffff;
+        s.place[k][b] = place;
+      }
+      atomicAdd(&s.bin_mass[b], m);
+      atomicAdd(&s.bin_count[b], c);
     }
     __syncthreads();
-    const int at = s.found;
-    before_count += at ? s.count[at - 1] : 0;
-    before_mass += at ? s.mass[at - 1] : 0;
-    prefix |= (uint32_t)at << next;
-    low = next;
+    uint32_t c = lane < kInGroup ? s.bin_count[lane] : 0;
+    u64 m = lane < kInGroup ? s.bin_mass[lane] : 0;
+    wave_scan(kInGroup, c, m);
+    votes = __ballot(lane < kInGroup && u.met(before_count + c, before_mass + m));
+    if (!votes) votes = __ballot(lane < kInGroup && c == __shfl(c, kInGroup - 1));
+    const int b = __ffsll(votes) - 1;
+    const uint32_t n = s.bin_count[b];
+    before_count += __shfl(c, b) - n;
+    before_mass += __shfl(m, b) - s.bin_mass[b];
+    // its tokens
+    const uint32_t place = lane < a.splits ? s.place[lane][b] : 0;
+    uint32_t upto = place & 0xffff;
+    u64 unused = 0;
+    wave_scan(kMaxSplits, upto, unused);
+    if (tid < kMaxSplits) s.upto[tid] = upto, s.begin[tid] = place >> 16;
     __syncthreads();
+    return n <= (uint32_t)kList ? in_list(u, n, before_count, before_mass) : in_buckets(u, n, before_count, before_mass);
   }
-  // ties: how many of this logit it takes, and which index that is
-  const uint32_t key = ~prefix;
-  const float logit = of_key(key);
-  const u64 w = Weigher::fixed(Weigher::weight(row.W.t(logit)));
-  uint32_t ties = 0;
-  {
-    u64 c = 0;
-    each_value<E, 4>(row.x, 0, row.vocab, tid, kPickThreads, AllValues{}, [&](int, float v) { c += v == logit; });
-    c = wave_reduce(c, [](u64 p, u64 q) { return p + q; });
-    if ((tid & 63) == 0) s.wave_count[tid >> 6] = (uint32_t)c;
-    __syncthreads();
-    for (int i = 0; i < kPickThreads / 64; ++i) ties += s.wave_count[i];
-    __syncthreads();
-  }
-  uint32_t lo = 1, hi = ties;  // the least n for which before + n of them meet `u`
-  while (lo < hi) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (u.met(before_count + mid, before_mass + mid * w)) hi = mid;
-    else lo = mid + 1;
-  }
-  // the lo-th index with this logit: pieces of the row in index order
-  if (tid == 0) s.found = 0;
-  uint32_t seen = 0;
-  for (int base = 0; base < row.vocab; base += kPickThreads) {
-    const int i = base + tid;
-    const bool hit = i < row.vocab && to_f32(row.x[i]) == logit;
-    const u64 votes = __ballot(hit);
-    if ((tid & 63) == 0) s.wave_count[tid >> 6] = __popcll(votes);
-    __syncthreads();
-    uint32_t mine = seen + __popcll(votes & ((2ull << (tid & 63)) - 1)), total = seen;
-    for (int v = 0; v < kPickThreads / 64; ++v) {
-      if (v < (tid >> 6)) mine += s.wave_count[v];
-      total += s.wave_count[v];
+
+  // Few: each token against all of them.
+  __device__ Found in_list(const Until &u, uint32_t n, uint32_t before_count, u64 before_mass) {
+    for (uint32_t j = threadIdx.x; j < n; j += kThreads) {
+      const int i = token(j);
+      const float v = to_f32(x[i]);
+      s.list[j] = Item{rank_of(key_of(v), i), mass_of(v)};
     }
-    if (hit && mine == lo) s.found = i;
     __syncthreads();
-    seen = total;
-    if (seen >= lo) break;
+    for (uint32_t j = threadIdx.x; j < n; j += kThreads) {
+      const Item own = s.list[j];
+      uint32_t c = before_count;
+      u64 m = before_mass;
+#pragma unroll 4
+      for (uint32_t k = 0; k < n; ++k) {
+        const Item o = s.list[k];
+        if (o.rank < own.rank) c += 1, m += o.mass;
+      }
+      if ((u.met(c + 1, m + own.mass) || c + 1 == before_count + n) && (c == before_count || !u.met(c, m)))
+        s.found = Found{own.rank, m + own.mass};
+    }
+    __syncthreads();
+    return s.found;
   }
-  const Found f{s.found, key, before_count + lo, before_mass + lo * w};
-  __syncthreads();
-  return f;
-}
+
+  // Many: the ranks' bits from the top, 11 at a time, in buckets that are counted and weighed.
+  __device__ Found in_buckets(const Until &u, uint32_t n, uint32_t before_count, u64 before_mass) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    u64 prefix = 0;
+    for (int low = 44; low >= 0; low -= 11) {
+      for (int i = tid; i < kBins; i += kThreads) s.mass[i] = 0, s.count[i] = 0;
+      if (tid == 0) s.bucket = kBins;
+      __syncthreads();
+      for (uint32_t j = tid; j < n; j += kThreads) {
+        const int i = token(j);
+        const float v = to_f32(x[i]);
+        const u64 r = rank_of(key_of(v), i);
+        if ((r ^ prefix) >> (low + 11)) continue;
+        const int at = (int)(r >> low) & (kBins - 1);
+        atomicAdd(&s.count[at], 1u);
+        atomicAdd(&s.mass[at], mass_of(v));
+      }
+      __syncthreads();
+      // running sums, four buckets a thread
+      uint32_t c[4], cs = 0;
+      u64 m[4], ms = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        cs += s.count[4 * tid + k];
+        ms += s.mass[4 * tid + k];
+        c[k] = cs;
+        m[k] = ms;
+      }
+      const uint32_t c_own = cs;
+      const u64 m_own = ms;
+      wave_scan(64, cs, ms);
+      if (lane == 63) s.wave_count[wave] = cs, s.wave_mass[wave] = ms;
+      __syncthreads();
+      uint32_t all = 0;
+      for (int w = 0; w < kThreads / 64; ++w) {
+        if (w < wave) cs += s.wave_count[w], ms += s.wave_mass[w];
+        all += s.wave_count[w];
+      }
+      cs += before_count - c_own;
+      ms += before_mass - m_own;
+#pragma unroll
+      for (int k = 3; k >= 0; --k)
+        if (s.count[4 * tid + k] && (u.met(cs + c[k], ms + m[k]) || cs + c[k] == before_count + all))
+          atomicMin(&s.bucket, 4u * tid + k);
+      __syncthreads();
+      const uint32_t at = s.bucket;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (at == 4u * tid + k) s.found = Found{cs + c[k] - s.count[at], ms + m[k] - s.mass[at]};  // what is before it
+      __syncthreads();
+      before_count = (uint32_t)s.found.rank;
+      before_mass = s.found.mass;
+      prefix |= (u64)at << low;
+      if (low == 0) before_mass += s.mass[at];
+      __syncthreads();
+    }
+    return Found{prefix, before_mass};
+  }
+};
 
 template <typename E>
-__global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
+__global__ __launch_bounds__(kThreads) void k_sample_pick(SampleArgs a) {
   __shared__ PickShared s;
   const int tid = threadIdx.x;
   const int64_t r = blockIdx.x;
@@ -497,52 +520,12 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
     }
     return;
   }
-  const Row<E> row{reinterpret_cast<const E *>(a.logits) + r * a.stride, a.vocab,
-                   Weigher(of_key((uint32_t)(best >> 32)), temp)};
-  // bins of the whole row, added up from its splits and scanned
-  auto whole_row = [&] {
-    for (int i = tid; i < kBins; i += kPickThreads) {
-      u64 m = 0;
-      uint32_t c = 0;
-#pragma unroll 8
-      for (int k = 0; k < a.splits; ++k) {
-        m += a.mass[(r * a.splits + k) * kBins + i];
-        c += a.count[(r * a.splits + k) * kBins + i];
-      }
-      s.mass[i] = m;
-      s.count[i] = c;
-    }
-    __syncthreads();
-    scan_bins(s);
-  };
-  whole_row();
-  int listed = 0, list_from = 1, list_to = 0;  // the list holds bins [list_from, list_to]
-  // The first token where `u` is met, or the last of all if none is.
-  auto find = [&](const Until &u) -> Found {
-    int b = first_bin(s, u);
-    if (b == kBins) b = first_bin(s, Until{Until::kCount, s.count[kBins - 1], 0.0});
-    auto before = [&](int x) { return x ? s.count[x - 1] : 0u; };
-    if (b < list_from || b > list_to) {
-      list_from = s.count[b] <= (uint32_t)kList ? 0 : b;
-      list_to = b;
-      if (s.count[b] - before(list_from) > (uint32_t)kList) {
-        const uint32_t c = before(b);
-        const u64 m = b ? s.mass[b - 1] : 0;
-        list_from = 1, list_to = 0;
-        __syncthreads();
-        const Found f = in_bin(s, row, b, u, c, m);
-        whole_row();
-        return f;
-      }
-      listed = gather(s, row, list_from, list_to);
-    }
-    return in_list(s, row, listed, u, before(list_from), list_from ? s.mass[list_from - 1] : 0);
-  };
-  u64 kept = s.mass[kBins - 1];
+  Pick<E> pick(a, s, r, Weigher(of_key((uint32_t)(best >> 32)), temp));
+  u64 kept = pick.weight();
   const int32_t top_k = a.top_ks ? a.top_ks[r] : a.top_k;
-  if (top_k > 0 && (uint32_t)top_k < s.count[kBins - 1]) kept = find(Until{Until::kCount, (uint32_t)top_k, 0.0}).mass;
+  if (top_k > 0 && (uint32_t)top_k < pick.tokens()) kept = pick.find(Until{Until::kCount, (uint32_t)top_k, 0.0}).mass;
   const float top_p = a.top_ps ? a.top_ps[r] : a.top_p;
-  if (top_p < 1.0f) kept = find(Until{Until::kAtLeast, 0, (double)top_p * (double)kept}).mass;
+  if (top_p < 1.0f) kept = pick.find(Until{Until::kAtLeast, 0, (double)top_p * (double)kept}).mass;
   u64 above = tid % 64 < a.splits ? a.min_mass[r * a.splits + tid % 64] : 0;
   above = wave_reduce(above, [](u64 p, u64 q) { return p + q; });
   const u64 first = (u64)kOne;
@@ -550,34 +533,50 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
   kept = above < kept ? above : kept;
   const float u = a.u[r];
   // the last kept token where u is 1 or more (or rounding would pass it), the first where u is negative or NaN
-  double goal = (u > 0.0f ? (double)u : 0.0) * (double)kept;
-  const Found f = goal < (double)kept ? find(Until{Until::kMore, 0, goal}) : find(Until{Until::kAtLeast, 0, (double)kept});
+  const double goal = (u > 0.0f ? (double)u : 0.0) * (double)kept;
+  const Found f = pick.find(goal < (double)kept ? Until{Until::kMore, 0, goal} : Until{Until::kAtLeast, 0, (double)kept});
   if (tid == 0) {
-    a.ids[r] = f.id;
-    if (a.probs) a.probs[r] = (float)(exp(-row.W.t(of_key(f.key))) / ((double)kept / kOne));
+    a.ids[r] = rank_index(f.rank);
+    if (a.probs) a.probs[r] = (float)(exp(-pick.W.t(of_key(rank_key(f.rank)))) / ((double)kept / kOne));
   }
 }
 
-// Tokens per split: at least 2048, so that the histograms cost less than the row.
-int splits_of(int64_t rows, int64_t vocab) {
-  int64_t n = (vocab + 2047) / 2048;
-  const int64_t enough = (2048 + rows - 1) / rows;  // 8 workgroups a CU
-  n = n < enough ? n : enough;
-  return (int)(n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n);
+// The splits of a row: of at most kPerSplit tokens, more of them where there are few rows.
+struct Split {
+  int splits, per_split;
+};
+Split split_of(int64_t rows, int64_t vocab) {
+  const int64_t least = (vocab + kPerSplit - 1) / kPerSplit, most = (vocab + 2047) / 2048;
+  int64_t n = (1024 + rows - 1) / rows;
+  n = n > most ? most : n;
+  n = n < least ? least : n;
+  n = n > kMaxSplits ? kMaxSplits : n;
+  const int64_t per = exl3h::align_up((size_t)((vocab + n - 1) / n), 8);
+  return Split{(int)((vocab + per - 1) / per), (int)per};
 }
 
 struct SampleWs {
-  size_t best, mass, count, min_mass, total;
+  size_t best, min_mass, mass, place, group_mass, group_count, order, total;
 };
 
 SampleWs sample_ws(int64_t rows, int64_t vocab) {
-  const size_t n = (size_t)rows * splits_of(rows, vocab);
+  const Split sp = split_of(rows, vocab);
+  const size_t n = (size_t)rows * sp.splits;
   SampleWs w;
-  w.best = 0;
-  w.min_mass = exl3h::align_up(n * 8, 256);
-  w.mass = w.min_mass + exl3h::align_up(n * 8, 256);
-  w.count = w.mass + n * kBins * 8;
-  w.total = w.count + n * kBins * 4;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += exl3h::align_up(bytes, 256);
+    return here;
+  };
+  w.best = take(n * 8);
+  w.min_mass = take(n * 8);
+  w.mass = take(n * kBins * 8);
+  w.place = take(n * kBins * 4);
+  w.group_mass = take(n * kGroups * 8);
+  w.group_count = take(n * kGroups * 4);
+  w.order = take(n * sp.per_split * 2);
+  w.total = at;
   return w;
 }
 
@@ -621,8 +620,9 @@ exl3_status exl3_sample(const exl3_sample_config *cfg, const void *logits, int64
   a.rows = rows;
   a.stride = row_stride;
   a.vocab = (int32_t)vocab;
-  a.splits = splits_of(rows, vocab);
-  a.per_split = (int32_t)((vocab + a.splits - 1) / a.splits);
+  const Split sp = split_of(rows, vocab);
+  a.splits = sp.splits;
+  a.per_split = sp.per_split;
   a.temperature = cfg->temperature;
   a.top_k = cfg->top_k;
   a.top_p = cfg->top_p;
@@ -638,14 +638,17 @@ exl3_status exl3_sample(const exl3_sample_config *cfg, const void *logits, int64
   a.best = reinterpret_cast<u64 *>(ws + w.best);
   a.min_mass = reinterpret_cast<u64 *>(ws + w.min_mass);
   a.mass = reinterpret_cast<u64 *>(ws + w.mass);
-  a.count = reinterpret_cast<uint32_t *>(ws + w.count);
+  a.place = reinterpret_cast<uint32_t *>(ws + w.place);
+  a.group_mass = reinterpret_cast<u64 *>(ws + w.group_mass);
+  a.group_count = reinterpret_cast<uint32_t *>(ws + w.group_count);
+  a.order = reinterpret_cast<uint16_t *>(ws + w.order);
   auto go = [&](auto e) {
     using E = decltype(e);
     const dim3 grid((unsigned)a.splits, (unsigned)rows);
     const hipStream_t st = stream_of(stream);
     k_sample_max<E><<<grid, kThreads, 0, st>>>(a);
-    if (cfg->temperatures || cfg->temperature > 0.0f) k_sample_hist<E><<<grid, kThreads, 0, st>>>(a);
-    k_sample_pick<E><<<(unsigned)rows, kPickThreads, 0, st>>>(a);
+    if (cfg->temperatures || cfg->temperature > 0.0f) k_sample_hist<E><<<grid, kThreads, 4 * (size_t)sp.per_split, st>>>(a);
+    k_sample_pick<E><<<(unsigned)rows, kThreads, 0, st>>>(a);
   };
   if (cfg->dtype == EXL3_ST_F32) go(float{});
   else with_elem16(cfg->dtype, go);
