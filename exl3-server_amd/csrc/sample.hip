@@ -50,6 +50,7 @@ constexpr int kMaxSplits = 64, kPerSplit = 8192;  // a lane per split; 13-bit pl
 constexpr int kNoBin = 0xffff;
 static_assert(kMaxT * kPerT < kBins, "every weighted token has a bin");
 static_assert(kMaxSplits * kPerSplit >= kMaxVocab, "the splits hold any row");
+static_assert(kPerSplit * 2 <= kBins * 8, "the indices fit where the weights were");
 static_assert(kThreads * 4 == kBins && kInGroup == 32, "four bins a thread, eight threads a group");
 
 typedef unsigned long long u64;
@@ -200,7 +201,6 @@ __global__ __launch_bounds__(kThreads) void k_sample_hist(SampleArgs a) {
   __shared__ uint32_t count[kBins];
   __shared__ u64 red[kThreads / 64];
   __shared__ uint32_t wave_count[kThreads / 64];
-  extern __shared__ __align__(16) uint16_t of_split[];  // per_split bins, then as many indices
   const int64_t row = blockIdx.y;
   const double temp = temperature_of(a, row);
   const u64 best = row_best(a, row);
@@ -213,9 +213,8 @@ __global__ __launch_bounds__(kThreads) void k_sample_hist(SampleArgs a) {
   const int first = min(a.vocab, (int)blockIdx.x * a.per_split), last = min(a.vocab, first + a.per_split);
   const E *x = reinterpret_cast<const E *>(a.logits) + row * a.stride;
   u64 above = 0;
-  each_value<E, 2>(x, first, last, tid, kThreads, [&](int i, float v) {
+  each_value<E, 2>(x, first, last, tid, kThreads, [&](int, float v) {
     const int b = W.bin(v);
-    of_split[i - first] = (uint16_t)b;
     if (b == kNoBin) return;
     const double w = W.weight(W.t(v));
     const u64 f = W.fixed(w);
@@ -268,12 +267,13 @@ __global__ __launch_bounds__(kThreads) void k_sample_hist(SampleArgs a) {
     a.min_mass[split] = above;
   }
   __syncthreads();
-  // the indices in the bins' order (within a bin in any)
-  uint16_t *ordered = of_split + a.per_split;
-  for (int i = tid; i < last - first; i += kThreads) {
-    const int b = of_split[i];
-    if (b != kNoBin) ordered[atomicAdd(&count[b], 1u)] = (uint16_t)i;
-  }
+  // the indices in the bins' order (within a bin in any), where the weights were: the bins are
+  // taken from the logits again, which costs less than the LDS to keep them (3 workgroups a CU)
+  uint16_t *ordered = reinterpret_cast<uint16_t *>(mass);
+  each_value<E, 2>(x, first, last, tid, kThreads, [&](int i, float v) {
+    const int b = W.bin(v);
+    if (b != kNoBin) ordered[atomicAdd(&count[b], 1u)] = (uint16_t)(i - first);
+  });
   __syncthreads();
   uint32_t all = 0;
   for (int w = 0; w < kThreads / 64; ++w) all += wave_count[w];
@@ -647,7 +647,7 @@ exl3_status exl3_sample(const exl3_sample_config *cfg, const void *logits, int64
     const dim3 grid((unsigned)a.splits, (unsigned)rows);
     const hipStream_t st = stream_of(stream);
     k_sample_max<E><<<grid, kThreads, 0, st>>>(a);
-    if (cfg->temperatures || cfg->temperature > 0.0f) k_sample_hist<E><<<grid, kThreads, 4 * (size_t)sp.per_split, st>>>(a);
+    if (cfg->temperatures || cfg->temperature > 0.0f) k_sample_hist<E><<<grid, kThreads, 0, st>>>(a);
     k_sample_pick<E><<<(unsigned)rows, kThreads, 0, st>>>(a);
   };
   if (cfg->dtype == EXL3_ST_F32) go(float{});
