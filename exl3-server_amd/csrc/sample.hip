@@ -339,18 +339,12 @@ struct Pick {
   uint32_t upto_count;  // this lane's group: tokens and weight up to and with it
   u64 upto_mass;
 
-  __device__ Pick(const SampleArgs &a, PickShared &s, int64_t row, const Weigher &W)
+  // (c, m): this thread's share of group tid % kGroups
+  __device__ Pick(const SampleArgs &a, PickShared &s, int64_t row, const Weigher &W, uint32_t c, u64 m)
       : a(a), s(s), row(row), x(reinterpret_cast<const E *>(a.logits) + row * a.stride), W(W) {
     const int tid = threadIdx.x, lane = tid & 63;
     if (tid < kGroups) s.group_mass[tid] = 0, s.group_count[tid] = 0;
     __syncthreads();
-    u64 m = 0;
-    uint32_t c = 0;
-#pragma unroll 8
-    for (int k = tid >> 6; k < a.splits; k += kThreads / 64) {
-      m += a.group_mass[(row * a.splits + k) * kGroups + lane];
-      c += a.group_count[(row * a.splits + k) * kGroups + lane];
-    }
     atomicAdd(&s.group_mass[lane], m);
     atomicAdd(&s.group_count[lane], c);
     __syncthreads();
@@ -414,8 +408,11 @@ struct Pick {
     // its tokens
     const uint32_t place = lane < a.splits ? s.place[lane][b] : 0;
     uint32_t upto = place & 0xffff;
-    u64 unused = 0;
-    wave_scan(kMaxSplits, upto, unused);
+#pragma unroll
+    for (int o = 1; o < kMaxSplits; o <<= 1) {
+      const uint32_t v = __shfl_up(upto, o);
+      if (lane >= o) upto += v;
+    }
     if (tid < kMaxSplits) s.upto[tid] = upto, s.begin[tid] = place >> 16;
     __syncthreads();
     return n <= (uint32_t)kList ? in_list(u, n, before_count, before_mass) : in_buckets(u, n, before_count, before_mass);
@@ -429,15 +426,26 @@ struct Pick {
       s.list[j] = Item{rank_of(key_of(v), i), mass_of(v)};
     }
     __syncthreads();
-    for (uint32_t j = threadIdx.x; j < n; j += kThreads) {
+    // as many lanes an item as there are threads for it (a power of two, in one wave)
+    int lanes = 64;
+    while (lanes > 1 && (uint32_t)lanes * n > (uint32_t)kThreads) lanes >>= 1;
+    for (uint32_t j = threadIdx.x / lanes; j < n; j += kThreads / lanes) {
       const Item own = s.list[j];
-      uint32_t c = before_count;
-      u64 m = before_mass;
+      uint32_t c = 0;
+      u64 m = 0;
 #pragma unroll 4
-      for (uint32_t k = 0; k < n; ++k) {
+      for (uint32_t k = threadIdx.x % lanes; k < n; k += lanes) {
         const Item o = s.list[k];
-        if (o.rank < own.rank) c += 1, m += o.mass;
+        const bool first = o.rank < own.rank;
+        c += first ? 1 : 0;
+        m += first ? o.mass : 0;
       }
+      for (int o = 1; o < lanes; o <<= 1) {
+        c += __shfl_xor(c, o);
+        m += __shfl_xor(m, o);
+      }
+      c += before_count;
+      m += before_mass;
       if ((u.met(c + 1, m + own.mass) || c + 1 == before_count + n) && (c == before_count || !u.met(c, m)))
         s.found = Found{own.rank, m + own.mass};
     }
@@ -510,8 +518,24 @@ __global__ __launch_bounds__(kThreads) void k_sample_pick(SampleArgs a) {
   __shared__ PickShared s;
   const int tid = threadIdx.x;
   const int64_t r = blockIdx.x;
-  const u64 best = row_best(a, r);
+  // everything that needs no other value first: a load that waits for one costs a microsecond
+  const int lane = tid & 63;
+  u64 best = lane < a.splits ? a.best[r * a.splits + lane] : 0;
+  u64 above = lane < a.splits ? a.min_mass[r * a.splits + lane] : 0;
   const double temp = temperature_of(a, r);
+  const int32_t top_k = a.top_ks ? a.top_ks[r] : a.top_k;
+  const float top_p = a.top_ps ? a.top_ps[r] : a.top_p;
+  const float u = a.u[r];
+  u64 m[kMaxSplits * 64 / kThreads];
+  uint32_t c[kMaxSplits * 64 / kThreads];
+#pragma unroll
+  for (int k = 0; k < kMaxSplits * 64 / kThreads; ++k) {
+    const int split = k * (kThreads / 64) + (tid >> 6);
+    const int64_t at = (r * a.splits + min(split, a.splits - 1)) * kGroups + lane;
+    m[k] = split < a.splits ? a.group_mass[at] : 0;
+    c[k] = split < a.splits ? a.group_count[at] : 0;
+  }
+  best = wave_reduce(best, [](u64 p, u64 q) { return p > q ? p : q; });
   const bool none = (uint32_t)(best >> 32) <= kMaskedKey;
   if (none || !(temp > 0.0)) {
     if (tid == 0) {
@@ -520,18 +544,16 @@ __global__ __launch_bounds__(kThreads) void k_sample_pick(SampleArgs a) {
     }
     return;
   }
-  Pick<E> pick(a, s, r, Weigher(of_key((uint32_t)(best >> 32)), temp));
+#pragma unroll
+  for (int k = 1; k < kMaxSplits * 64 / kThreads; ++k) m[0] += m[k], c[0] += c[k];
+  Pick<E> pick(a, s, r, Weigher(of_key((uint32_t)(best >> 32)), temp), c[0], m[0]);
   u64 kept = pick.weight();
-  const int32_t top_k = a.top_ks ? a.top_ks[r] : a.top_k;
   if (top_k > 0 && (uint32_t)top_k < pick.tokens()) kept = pick.find(Until{Until::kCount, (uint32_t)top_k, 0.0}).mass;
-  const float top_p = a.top_ps ? a.top_ps[r] : a.top_p;
   if (top_p < 1.0f) kept = pick.find(Until{Until::kAtLeast, 0, (double)top_p * (double)kept}).mass;
-  u64 above = tid % 64 < a.splits ? a.min_mass[r * a.splits + tid % 64] : 0;
   above = wave_reduce(above, [](u64 p, u64 q) { return p + q; });
   const u64 first = (u64)kOne;
   above = above < first ? first : above;
   kept = above < kept ? above : kept;
-  const float u = a.u[r];
   // the last kept token where u is 1 or more (or rounding would pass it), the first where u is negative or NaN
   const double goal = (u > 0.0f ? (double)u : 0.0) * (double)kept;
   const Found f = pick.find(goal < (double)kept ? Until{Until::kMore, 0, goal} : Until{Until::kAtLeast, 0, (double)kept});
