@@ -590,11 +590,16 @@ __device__ __forceinline__ void put_split(f16 *hi, f16 *lo, const float (&v)[N],
 // there (and its values), in the other of two buffers, and load the one after it: the
 // multiplying waves wait for no load, and their stores are never waited for.
 template <typename E, int DK, bool kChannel, int kWaves>
-__global__ __launch_bounds__(64 * kWaves + 256) void k_delta_scan(DeltaArgs a) {
+__global__ __launch_bounds__(64 * kWaves + 256) void k_delta_scan(DeltaArgs a, int parts) {
   constexpr int N = DK / 64, KT = DK / 16;
   using St = Stage<E, DK, kWaves>;
   __shared__ St stage[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seq = blockIdx.z, h = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // Workgroups go to the 8 XCDs in turn: the `parts` column blocks of one head and sequence
+  // to one XCD, whose L2 then reads the rows they share once.
+  const int turn = blockIdx.x / 8, part_of = turn % parts, pair = turn / parts * 8 + blockIdx.x % 8;
+  if (pair >= a.heads_v * a.n_seq) return;
+  const int seq = pair / a.heads_v, h = pair % a.heads_v;
   const int hk = h / (a.heads_v / a.heads_qk), g = lane / 16, m = lane % 16;
   const int64_t from = slot_of(a.src, seq, a.n_slots), to = slot_of(a.dst, seq, a.n_slots);
   const bool write = sole_writer(a, seq, to);
@@ -612,7 +617,7 @@ __global__ __launch_bounds__(64 * kWaves + 256) void k_delta_scan(DeltaArgs a) {
     // 8 values of a row; kPieces such pieces are the workgroup's columns
     typedef E E8 __attribute__((ext_vector_type(8), aligned(2)));
     constexpr int kPieces = kWaves * kCols / 8;
-    const uint32_t v_col = blockIdx.x * kWaves * kCols + part % kPieces * 8;
+    const uint32_t v_col = part_of * kWaves * kCols + part % kPieces * 8;
     const bool has_v = part < kC * kPieces && (int)v_col < a.dv;
     E8 val;
 #pragma unroll
@@ -704,8 +709,8 @@ __global__ __launch_bounds__(64 * kWaves + 256) void k_delta_scan(DeltaArgs a) {
     return;
   }
 
-  const int col = (blockIdx.x * kWaves + wave) * kCols + m;
-  if ((blockIdx.x * kWaves + wave) * kCols >= a.dv) {  // only keeps step
+  const int col = (part_of * kWaves + wave) * kCols + m;
+  if ((part_of * kWaves + wave) * kCols >= a.dv) {  // only keeps step
     for (int c = 0; c <= chunks; ++c) lds_barrier();
     return;
   }
@@ -998,8 +1003,9 @@ exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows 
         // sequences of up to 1001 tokens of 32 heads 119 against 94 us.
         auto scan = [&](auto waves) {
           constexpr int kWaves = decltype(waves)::value;
-          const dim3 blocks((unsigned)((cfg->dv / kCols + kWaves - 1) / kWaves), (unsigned)cfg->heads_v, (unsigned)n_seq);
-          k_delta_scan<E, DK, kChannel, kWaves><<<blocks, 64 * kWaves + 256, 0, st>>>(a);
+          const int parts = (cfg->dv / kCols + kWaves - 1) / kWaves;
+          const unsigned blocks = (unsigned)((cfg->heads_v * n_seq + 7) / 8 * 8 * parts);
+          k_delta_scan<E, DK, kChannel, kWaves><<<blocks, 64 * kWaves + 256, 0, st>>>(a, parts);
         };
         if ((cfg->dv / kCols + 1) / 2 * (int64_t)cfg->heads_v * n_seq <= 256) scan(std::integral_constant<int, 2>{});
         else scan(std::integral_constant<int, 4>{});
