@@ -304,181 +304,10 @@ __device__ __forceinline__ void put(float *p, const float (&v)[N]) {
   if constexpr (N == 2) *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]);
   else *p = v[0];
 }
-template <int N>
-__device__ __forceinline__ void put_scaled(float *p, const float (&v)[N], const float (&s)[N]) {
-  float x[N];
-#pragma unroll
-  for (int n = 0; n < N; ++n) x[n] = v[n] * s[n];
-  put<N>(p, x);
-}
-
 __device__ __forceinline__ f32x4 mfma4(const f32x4 &a, const f32x4 &b, f32x4 c) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
   return c;
-}
-
-// T and B of one chunk and value head. For each h = 1, 2, 4, 8, 16 the pairs (i, j) whose
-// highest differing bit is h: i in the later half of a block of 2 h tokens, j in the earlier
-// one, so P_i / P_j = (product from the halves' border to i) (product from j to the border),
-// both at most 1 for decays that are. The 16 rows with bit h and the 16 without it are one
-// tile of the matrix instruction, of which the pairs of a common block are taken.
-template <typename E, int DK, bool kChannel>
-__global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a) {
-  constexpr int N = DK / 64, kRow = DK + kPad;
-  __shared__ float left_k[16 * kRow], left_q[16 * kRow], right[16 * kRow];
-  __shared__ float total[4][DK];
-  __shared__ float sum[2][5][256];             // the second halves of the channels
-  __shared__ float A[kC][kC + kPad], B[kC][kC + kPad];
-  __shared__ float beta[kC], diag[kC];
-  __shared__ int seq;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, id = blockIdx.x, h = blockIdx.y;
-  if (tid == 0) seq = a.n_seq;
-  __syncthreads();
-  for (int i = tid; i < a.n_seq; i += 256) {
-    const Seq s = seq_of(a, i);
-    const int c = id - first_chunk(s, i);
-    if (c >= 0 && c < chunks_of(s)) atomicMin(&seq, i);
-  }
-  __syncthreads();
-  if (seq == a.n_seq) return;
-  const Seq s = seq_of(a, seq);
-  const int t0 = uniform(s.first + (id - first_chunk(s, seq)) * kC), n = uniform(s.last) - t0;
-  RawSlice<E, DK, kChannel> raw;
-  raw.load(a, t0, n, h, h / (a.heads_v / a.heads_qk), 8 * wave, lane * N);
-  float b = 0.0f;
-  if (tid < kC) {
-    b = tid < n ? a.beta[(int64_t)(t0 + tid) * a.beta_token + h] : 0.0f;
-    beta[tid] = b;
-  }
-  Slice<E, DK, kChannel> x;
-  if (n < kC) raw.clear(n, 8 * wave);
-  x.convert(raw);
-  const bool fine = !__syncthreads_or(!x.fine() || !(b * 0.0f == 0.0f));
-  // B's diagonal
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float d = 0.0f;
-#pragma unroll
-    for (int n = 0; n < N; ++n) d = fmaf(x.q[i][n], x.k[i][n], d);
-    d += xor_lanes<1>(d);
-    d += xor_lanes<2>(d);
-    d += xor_lanes<4>(d);
-    d += xor_lanes<8>(d);
-    d += xor_lanes<16>(d);
-    d += xor_lanes<32>(d);
-    if (lane == 0) diag[8 * wave + i] = d;
-  }
-  f32x4 acc[5];
-#pragma unroll
-  for (int level = 0; level < 5; ++level) {
-    const int hh = 1 << level;
-    if (level) __syncthreads();  // the tile's last operands are read
-    if (hh < 8) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int row = (8 * wave + i) / (2 * hh) * hh + (i & (hh - 1));  // without bit h
-        float *at = (i & hh ? left_k : right) + row * kRow + lane * N;
-        if (i & hh) {
-          put_scaled<N>(at, x.k[i], x.P[i]);
-          put_scaled<N>(left_q + row * kRow + lane * N, x.q[i], x.P[i]);
-        } else {
-          put_scaled<N>(at, x.k[i], x.X[i]);
-        }
-      }
-    } else {
-      const bool later = wave & (hh / 8);
-      const int first = hh == 8 ? wave / 2 * 8 : wave % 2 * 8;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (later) {
-          put_scaled<N>(left_k + (first + i) * kRow + lane * N, x.k[i], x.P[i]);
-          put_scaled<N>(left_q + (first + i) * kRow + lane * N, x.q[i], x.P[i]);
-        } else {
-          put_scaled<N>(right + (first + i) * kRow + lane * N, x.k[i], x.X[i]);
-        }
-      }
-    }
-    if (hh < 8) x.grow(hh);
-    if (hh == 4) put<N>(&total[wave][lane * N], x.P[7]);
-    __syncthreads();
-    // waves 0, 1: A and B over the first half of the channels, waves 2, 3 over the second
-    const float *l = (wave & 1 ? left_q : left_k) + lane % 16 * kRow + lane / 16 * 4;
-    const float *r = right + lane % 16 * kRow + lane / 16 * 4;
-    f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int kt = 0; kt < DK / 32; ++kt) {
-      const int k0 = (wave >> 1) * (DK / 2) + 16 * kt;
-      c = mfma4(*reinterpret_cast<const f32x4 *>(l + k0), *reinterpret_cast<const f32x4 *>(r + k0), c);
-    }
-    acc[level] = c;
-    if (hh == 8) {  // to blocks of 16
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-          const float t = total[wave ^ 1][lane * N + n];
-          if (wave & 1) x.P[i][n] *= t;
-          else x.X[i][n] *= t;
-        }
-    }
-  }
-  if (wave >= 2) {
-#pragma unroll
-    for (int level = 0; level < 5; ++level)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) sum[wave & 1][level][r * 64 + lane] = acc[level][r];
-  }
-  for (int i = tid; i < kC * kC; i += 256) {  // on and over the diagonal
-    const int row = i / kC, col = i % kC;
-    if (col >= row) A[row][col] = 0.0f, B[row][col] = col == row ? diag[row] : 0.0f;
-  }
-  __syncthreads();
-  if (wave < 2) {
-    float(*to)[kC + kPad] = wave ? B : A;
-#pragma unroll
-    for (int level = 0; level < 5; ++level)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int hh = 1 << level, ic = lane / 16 * 4 + r, jc = lane % 16;
-        const int i = ic / hh * 2 * hh + hh + ic % hh, j = jc / hh * 2 * hh + jc % hh;
-        if (ic / hh == jc / hh) to[i][j] = acc[level][r] + sum[wave][level][r * 64 + lane];
-      }
-  }
-  __syncthreads();
-  ChunkMats &out = a.chunks[(size_t)id * a.heads_v + h];
-  auto put_split = [&](int which, int i, int j, float v) {
-    const float y = f32_rounded(v * kScale);
-    const f16 hi = (f16)y;
-    out.mat[which][i][in_order(j)] = hi;
-    out.mat[which + 1][i][in_order(j)] = (f16)(y - (float)hi);
-  };
-  if (wave == 0) {
-    // column `lane` of T by forward substitution
-    float t[kC], most = 0.0f;
-    if (lane < kC) {
-#pragma unroll
-      for (int i = 0; i < kC; ++i) {
-        float v = 0.0f;
-#pragma unroll
-        for (int l = 0; l < i; ++l) v = fmaf(A[i][l], t[l], v);
-        t[i] = beta[i] * ((i == lane ? 1.0f : 0.0f) - v);
-        most = fmaxf(most, fabsf(t[i]));
-        put_split(0, i, lane, t[i]);
-      }
-    }
-    const bool large = __any(!(most < kLimit));
-    if (lane == 0) out.fine[0] = fine && !large;
-  } else if (wave == 1) {
-    float most = 0.0f;
-    for (int i = lane; i < kC * kC; i += 64) {
-      const float v = B[i / kC][i % kC];
-      most = fmaxf(most, fabsf(v));
-      put_split(2, i / kC, i % kC, v);
-    }
-    const bool large = __any(!(most < kLimit));
-    if (lane == 0) out.fine[1] = !large;
-  }
 }
 
 // A barrier that orders LDS alone: __syncthreads() would also wait for every global load and
@@ -579,6 +408,228 @@ __device__ __forceinline__ void put_split(f16 *hi, f16 *lo, const float (&v)[N],
     }
     *reinterpret_cast<words *>(hi) = wh;
     *reinterpret_cast<words *>(lo) = wl;
+  }
+}
+
+// Sums over the wave of 8 values a lane: lane 16 r holds those of value r / 2 * 4 + r % 2 * 2 + i in
+// v[i], i = 0, 1. Halves and rows are exchanged with half of the values each, so that
+// each step halves what is left.
+__device__ __forceinline__ void wave_sums8(float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const auto r = __builtin_amdgcn_permlane32_swap(bitcast<uint32_t>(v[i]), bitcast<uint32_t>(v[i + 4]), false, false);
+    v[i] = bitcast<float>(r[0]) + bitcast<float>(r[1]);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const auto r = __builtin_amdgcn_permlane16_swap(bitcast<uint32_t>(v[i]), bitcast<uint32_t>(v[i + 2]), false, false);
+    v[i] = bitcast<float>(r[0]) + bitcast<float>(r[1]);
+    // lanes ^ 1, ^ 2, and the mirrors of 8 and of 16 lanes
+    v[i] += bitcast<float>(__builtin_amdgcn_mov_dpp(bitcast<int>(v[i]), 0xB1, 0xF, 0xF, false));
+    v[i] += bitcast<float>(__builtin_amdgcn_mov_dpp(bitcast<int>(v[i]), 0x4E, 0xF, 0xF, false));
+    v[i] += bitcast<float>(__builtin_amdgcn_mov_dpp(bitcast<int>(v[i]), 0x141, 0xF, 0xF, false));
+    v[i] += bitcast<float>(__builtin_amdgcn_mov_dpp(bitcast<int>(v[i]), 0x140, 0xF, 0xF, false));
+  }
+}
+
+// T and B of one chunk and value head. For each h = 1, 2, 4, 8, 16 the pairs (i, j) whose
+// highest differing bit is h: i in the later half of a block of 2 h tokens, j in the earlier
+// one, so P_i / P_j = (product from the halves' border to i) (product from j to the border),
+// both at most 1 for decays that are. The 16 rows with bit h and the 16 without it are one
+// tile of the matrix instruction, of which the pairs of a common block are taken. Waves 0
+// and 1 multiply A's and B's tiles of h = 1, 4, 16, waves 2 and 3 those of 2 and 8.
+template <typename E, int DK, bool kChannel>
+__global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a) {
+  constexpr int N = DK / 64, kRow = DK + 8;
+  struct Operands {
+    f16 left_k[2][16][kRow], left_q[2][16][kRow], right[2][16][kRow];  // hi, lo, times 2^6
+  };
+  struct Results {
+    float A[kC][kC + kPad], B[kC][kC + kPad];
+    float t00[16][16 + kPad], m11[16][16 + kPad];  // columns
+  };
+  union Lds {
+    Operands in;
+    Results out;
+  };
+  __shared__ Lds lds;
+  __shared__ float total[4][DK];
+  __shared__ float beta[kC], diag[kC];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, id = blockIdx.x, h = blockIdx.y;
+  int seq = 0;
+  if (a.n_seq > 1) {
+    __shared__ int of;
+    if (tid == 0) of = a.n_seq;
+    __syncthreads();
+    for (int i = tid; i < a.n_seq; i += 256) {
+      const Seq s = seq_of(a, i);
+      const int c = id - first_chunk(s, i);
+      if (c >= 0 && c < chunks_of(s)) atomicMin(&of, i);
+    }
+    __syncthreads();
+    seq = of;
+    if (seq == a.n_seq) return;
+  }
+  const Seq s = seq_of(a, seq);
+  const int chunk = id - first_chunk(s, seq);
+  if (chunk < 0 || chunk >= chunks_of(s)) return;
+  const int t0 = uniform(s.first + chunk * kC), n = uniform(s.last) - t0;
+  RawSlice<E, DK, kChannel> raw;
+  raw.load(a, t0, n, h, h / (a.heads_v / a.heads_qk), 8 * wave, lane * N);
+  float b = 0.0f;
+  if (tid < kC) {
+    b = tid < n ? a.beta[(int64_t)(t0 + tid) * a.beta_token + h] : 0.0f;
+    beta[tid] = b;
+  }
+  if (n < kC) raw.clear(n, 8 * wave);
+  Slice<E, DK, kChannel> x;
+  x.convert(raw);
+  const bool fine = !__syncthreads_or(!x.fine() || !(b * 0.0f == 0.0f));
+  {  // B's diagonal
+    float d[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      d[i] = x.q[i][0] * x.k[i][0];
+      if constexpr (N == 2) d[i] = fmaf(x.q[i][1], x.k[i][1], d[i]);
+    }
+    wave_sums8(d);
+    const int row = lane / 16;
+    if (lane % 16 < 2) diag[8 * wave + row / 2 * 4 + row % 2 * 2 + lane % 16] = lane % 16 ? d[1] : d[0];
+  }
+  // times 2^6 on both sides of a tile
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int c = 0; c < N; ++c) x.k[i][c] *= kScale, x.q[i][c] *= kScale;
+  f32x4 acc[3];
+#pragma unroll
+  for (int level = 0; level < 5; ++level) {
+    const int hh = 1 << level;
+    if (level) __syncthreads();  // the last tile's operands are read
+    auto put_left = [&](int row, int i) {
+      put_split<N>(&lds.in.left_k[0][row][lane * N], &lds.in.left_k[1][row][lane * N], x.k[i], x.P[i]);
+      put_split<N>(&lds.in.left_q[0][row][lane * N], &lds.in.left_q[1][row][lane * N], x.q[i], x.P[i]);
+    };
+    auto put_right = [&](int row, int i) {
+      put_split<N>(&lds.in.right[0][row][lane * N], &lds.in.right[1][row][lane * N], x.k[i], x.X[i]);
+    };
+    if (hh < 8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = (8 * wave + i) / (2 * hh) * hh + (i & (hh - 1));  // without bit h
+        if (i & hh) put_left(row, i);
+        else put_right(row, i);
+      }
+    } else {
+      const int first = hh == 8 ? wave / 2 * 8 : wave % 2 * 8;
+      if (wave & (hh / 8)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) put_left(first + i, i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) put_right(first + i, i);
+      }
+    }
+    if (hh < 8) x.grow(hh);
+    if (hh == 4) put<N>(&total[wave][lane * N], x.P[7]);
+    __syncthreads();
+    if (wave / 2 == level % 2) {
+      auto operand = [&](const f16(&p)[2][16][kRow], int k0) {
+        return Pair{*reinterpret_cast<const f16x8 *>(&p[0][lane % 16][k0 + lane / 16 * 8]),
+                    *reinterpret_cast<const f16x8 *>(&p[1][lane % 16][k0 + lane / 16 * 8])};
+      };
+      Pair l[DK / 32][1], r[DK / 32];
+#pragma unroll
+      for (int k = 0; k < DK / 32; ++k) {
+        l[k][0] = wave & 1 ? operand(lds.in.left_q, 32 * k) : operand(lds.in.left_k, 32 * k);
+        r[k] = operand(lds.in.right, 32 * k);
+      }
+      f32x4 c[1] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+      product<DK / 32, 1>(l, r, c);
+      acc[level / 2] = c[0];
+    }
+    if (hh == 8) {  // to blocks of 16
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+          const float t = total[wave ^ 1][lane * N + c];
+          if (wave & 1) x.P[i][c] *= t;
+          else x.X[i][c] *= t;
+        }
+    }
+  }
+  __syncthreads();
+  // every element under the diagonal is in one level's tile
+  {
+    float(*to)[kC + kPad] = wave & 1 ? lds.out.B : lds.out.A;
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int hh = 1 << (2 * k + wave / 2), ic = lane / 16 * 4 + r, jc = lane % 16;
+        const int i = ic / hh * 2 * hh + hh + ic % hh, j = jc / hh * 2 * hh + jc % hh;
+        if (hh <= 16 && ic / hh == jc / hh) to[i][j] = acc[k][r] * (1.0f / (kScale * kScale));
+      }
+  }
+  __syncthreads();
+  ChunkMats &out = a.chunks[(size_t)id * a.heads_v + h];
+  auto put_out = [&](int which, int i, int j, float v) {
+    f16x2 hi, lo;
+    split2(v, kScale, 0.0f, 0.0f, hi, lo);
+    out.mat[which][i][in_order(j)] = hi[0];
+    out.mat[which + 1][i][in_order(j)] = lo[0];
+  };
+  if (wave == 0) {
+    // (I + diag(beta) A)^-1 in blocks of 16: lanes 0 to 15 the columns of the first, 16 to 31 those
+    // of the second by forward substitution, then -M11 N10 M00 as two small products
+    const int col = lane % 16, g = lane / 16, block = g & 1;
+    float t[16], most = 0.0f;
+    const float bj = beta[16 * block + col];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float v = 0.0f;
+#pragma unroll
+      for (int l = 0; l < i; ++l) v = fmaf(lds.out.A[16 * block + i][16 * block + l], t[l], v);
+      t[i] = (i == col ? 1.0f : 0.0f) - beta[16 * block + i] * v;
+    }
+    if (lane < 32) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float v = t[i] * bj;
+        (block ? lds.out.m11 : lds.out.t00)[col][i] = block ? t[i] : v;
+        most = fmaxf(most, fabsf(v));
+        put_out(0, 16 * block + i, 16 * block + col, v);
+        if (!block) put_out(0, i, 16 + col, 0.0f);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f}, z = y, m;
+    y = mfma4(*reinterpret_cast<const f32x4 *>(&lds.out.A[16 + col][4 * g]),
+              *reinterpret_cast<const f32x4 *>(&lds.out.t00[col][4 * g]), y);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      y[r] *= -beta[16 + 4 * g + r];
+      m[r] = lds.out.m11[4 * g + r][col];
+    }
+    z = mfma4(m, y, z);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      most = fmaxf(most, fabsf(z[r]));
+      put_out(0, 16 + 4 * g + r, col, z[r]);
+    }
+    const bool large = __any(!(most < kLimit));
+    if (lane == 0) out.fine[0] = fine && !large;
+  } else if (wave == 1) {
+    float most = 0.0f;
+    for (int i = lane; i < kC * kC; i += 64) {
+      const int row = i / kC, c = i % kC;
+      const float v = c > row ? 0.0f : c == row ? diag[row] : lds.out.B[row][c];
+      most = fmaxf(most, fabsf(v));
+      put_out(2, row, c, v);
+    }
+    const bool large = __any(!(most < kLimit));
+    if (lane == 0) out.fine[1] = !large;
   }
 }
 
