@@ -271,13 +271,23 @@ struct Slice {
         X[i][c] = 1.0f;
       }
   }
-  // Whether the scan may multiply these values (neither does any NaN pass).
-  __device__ __forceinline__ bool fine() const {
-    bool ok = true;
+  // Whether the scan may multiply these values, by their bits: magnitudes order as integers,
+  // infinities and NaN above all others.
+  __device__ __forceinline__ bool fine(const RawSlice<E, DK, kChannel> &x) const {
+    typedef uint16_t U __attribute__((ext_vector_type(N)));
+    U most = 0;
+    uint32_t decay = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 8; ++i) {
+      most = __builtin_elementwise_max(most, __builtin_elementwise_max((U)(bitcast<U>(x.k[i]) & (uint16_t)0x7fff),
+                                                                       (U)(bitcast<U>(x.q[i]) & (uint16_t)0x7fff)));
 #pragma unroll
-      for (int n = 0; n < N; ++n) ok = ok && fabsf(k[i][n]) < kLimit && fabsf(q[i][n]) < kLimit && P[i][n] <= 1.0f;
+      for (int n = 0; n < N; ++n) decay = max(decay, bitcast<uint32_t>(P[i][n]));
+    }
+    const uint16_t limit = bitcast<uint16_t>(from_f32<E>(kLimit));
+    bool ok = decay <= 0x3f800000u;  // 1.0f
+#pragma unroll
+    for (int n = 0; n < N; ++n) ok = ok && most[n] < limit;
     return ok;
   }
   // from blocks of h to blocks of 2 h tokens (h = 1, 2, 4)
@@ -439,7 +449,7 @@ __device__ __forceinline__ void wave_sums8(float (&v)[8]) {
 // tile of the matrix instruction, of which the pairs of a common block are taken. Waves 0
 // and 1 multiply A's and B's tiles of h = 1, 4, 16, waves 2 and 3 those of 2 and 8.
 template <typename E, int DK, bool kChannel>
-__global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a) {
+__global__ __launch_bounds__(256, 4) void k_delta_chunk(DeltaArgs a) {
   constexpr int N = DK / 64, kRow = DK + 8;
   struct Operands {
     f16 left_k[2][16][kRow], left_q[2][16][kRow], right[2][16][kRow];  // hi, lo, times 2^6
@@ -447,6 +457,8 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a) {
   struct Results {
     float A[kC][kC + kPad], B[kC][kC + kPad];
     float t00[16][16 + kPad], m11[16][16 + kPad];  // columns
+    f16 mat[4][kC][kC];                            // as ChunkMats
+    int fine[2];
   };
   union Lds {
     Operands in;
@@ -484,7 +496,7 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a) {
   if (n < kC) raw.clear(n, 8 * wave);
   Slice<E, DK, kChannel> x;
   x.convert(raw);
-  const bool fine = !__syncthreads_or(!x.fine() || !(b * 0.0f == 0.0f));
+  const bool fine = !__syncthreads_or(!x.fine(raw) || !(b * 0.0f == 0.0f));
   {  // B's diagonal
     float d[8];
 #pragma unroll
@@ -573,12 +585,11 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a) {
       }
   }
   __syncthreads();
-  ChunkMats &out = a.chunks[(size_t)id * a.heads_v + h];
   auto put_out = [&](int which, int i, int j, float v) {
     f16x2 hi, lo;
     split2(v, kScale, 0.0f, 0.0f, hi, lo);
-    out.mat[which][i][in_order(j)] = hi[0];
-    out.mat[which + 1][i][in_order(j)] = lo[0];
+    lds.out.mat[which][i][in_order(j)] = hi[0];
+    lds.out.mat[which + 1][i][in_order(j)] = lo[0];
   };
   if (wave == 0) {
     // (I + diag(beta) A)^-1 in blocks of 16: lanes 0 to 15 the columns of the first, 16 to 31 those
@@ -592,6 +603,7 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a) {
 #pragma unroll
       for (int l = 0; l < i; ++l) v = fmaf(lds.out.A[16 * block + i][16 * block + l], t[l], v);
       t[i] = (i == col ? 1.0f : 0.0f) - beta[16 * block + i] * v;
+      if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (else all rows are read at once, into registers)
     }
     if (lane < 32) {
 #pragma unroll
@@ -600,7 +612,6 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a) {
         (block ? lds.out.m11 : lds.out.t00)[col][i] = block ? t[i] : v;
         most = fmaxf(most, fabsf(v));
         put_out(0, 16 * block + i, 16 * block + col, v);
-        if (!block) put_out(0, i, 16 + col, 0.0f);
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -619,7 +630,7 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a) {
       put_out(0, 16 + 4 * g + r, col, z[r]);
     }
     const bool large = __any(!(most < kLimit));
-    if (lane == 0) out.fine[0] = fine && !large;
+    if (lane == 0) lds.out.fine[0] = fine && !large;
   } else if (wave == 1) {
     float most = 0.0f;
     for (int i = lane; i < kC * kC; i += 64) {
@@ -629,8 +640,18 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a) {
       put_out(2, row, c, v);
     }
     const bool large = __any(!(most < kLimit));
-    if (lane == 0) out.fine[1] = !large;
+    if (lane == 0) lds.out.fine[1] = !large;
+  } else if (wave == 2) {
+    // T over its diagonal blocks
+#pragma unroll
+    for (int k = 0; k < 4; ++k) put_out(0, 4 * k + lane / 16, 16 + lane % 16, 0.0f);
   }
+  __syncthreads();
+  ChunkMats &out = a.chunks[(size_t)id * a.heads_v + h];
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    reinterpret_cast<u32x4 *>(out.mat)[tid + 256 * k] = reinterpret_cast<const u32x4 *>(lds.out.mat)[tid + 256 * k];
+  if (tid < 2) out.fine[tid] = lds.out.fine[tid];
 }
 
 // A sequence's chunks in turn. The first kWaves waves hold kCols columns of the state each, as the
