@@ -75,16 +75,25 @@ __device__ __forceinline__ bool sole_writer(const DeltaArgs &a, int i, int64_t s
   return !__syncthreads_or(met) && slot >= 0;
 }
 
-// Sum over the 16 lanes of a wave that hold the same columns (lane / 4).
+// x + the partner's x, of lane ^ 16 and of lane ^ 32: an exchange holds both, in either order.
+__device__ __forceinline__ float add_16(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(bitcast<uint32_t>(x), bitcast<uint32_t>(x), false, false);
+  return bitcast<float>(r[0]) + bitcast<float>(r[1]);
+}
+__device__ __forceinline__ float add_32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(bitcast<uint32_t>(x), bitcast<uint32_t>(x), false, false);
+  return bitcast<float>(r[0]) + bitcast<float>(r[1]);
+}
+
+// Sum over the 16 lanes of a wave that hold the same columns (lane / 4), the same bits in all:
+// rows of 16 lanes turned by 8 (lane ^ 8), by 4 (as lane ^ 4 then), and the rows. No LDS.
 __device__ __forceinline__ f32x4 sum_rows(f32x4 v) {
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     float x = v[c];
-    x += xor_lanes<4>(x);
-    x += xor_lanes<8>(x);
-    x += xor_lanes<16>(x);
-    x += xor_lanes<32>(x);
-    v[c] = x;
+    x += bitcast<float>(__builtin_amdgcn_mov_dpp(bitcast<int>(x), 0x128, 0xF, 0xF, false));
+    x += bitcast<float>(__builtin_amdgcn_mov_dpp(bitcast<int>(x), 0x124, 0xF, 0xF, false));
+    v[c] = add_32(add_16(x));
   }
   return v;
 }
@@ -112,18 +121,37 @@ __global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a) {
   const E *v = reinterpret_cast<const E *>(a.v) + (int64_t)h * a.dv + col;
   E *out = reinterpret_cast<E *>(a.out) + (int64_t)h * a.dv + col;
   const float *g = a.g + (kChannel ? (int64_t)h * DK + row : h);
+  // a token's rows, the next one's loaded while this one's are computed on
+  typedef E ER __attribute__((ext_vector_type(R), aligned(2)));
+  typedef E E4 __attribute__((ext_vector_type(4), aligned(2)));
+  typedef float GR __attribute__((ext_vector_type(kChannel ? R : 1), aligned(4)));
+  struct Token {
+    ER k, q;
+    GR g;
+    E4 v;
+    float beta;
+  };
+  auto load = [&](int64_t t) {
+    return Token{*reinterpret_cast<const ER *>(k + t * a.k_token), *reinterpret_cast<const ER *>(q + t * a.q_token),
+                 *reinterpret_cast<const GR *>(g + t * a.g_token), *reinterpret_cast<const E4 *>(v + t * a.v_token),
+                 a.beta[t * a.beta_token + h]};
+  };
+  Token next;
+  if (s.first < s.last) next = load(s.first);
   for (int64_t t = s.first; t < s.last; ++t) {
+    const Token now = next;
+    next = load(t + 1 < s.last ? t + 1 : t);
     float kk[R], qq[R], decay[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      kk[r] = to_f32(k[t * a.k_token + r]);
-      qq[r] = to_f32(q[t * a.q_token + r]);
-      decay[r] = g[t * a.g_token + (kChannel ? r : 0)];
+      kk[r] = to_f32((E)now.k[r]);
+      qq[r] = to_f32((E)now.q[r]);
+      decay[r] = now.g[kChannel ? r : 0];
     }
-    const float beta = a.beta[t * a.beta_token + h];
+    const float beta = now.beta;
     f32x4 vv;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) vv[c] = to_f32(v[t * a.v_token + c]);
+    for (int c = 0; c < 4; ++c) vv[c] = to_f32((E)now.v[c]);
     f32x4 dot = {0.0f, 0.0f, 0.0f, 0.0f}, o = dot;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -827,8 +855,7 @@ __global__ __launch_bounds__(64 * kWaves + 256) void k_delta_scan(DeltaArgs a, i
           S[kt][r] *= decay_of(gp[kChannel ? ch : 0]);
           dot = fmaf(to_f32(k[ch]), S[kt][r], dot);
         }
-      dot += xor_lanes<16>(dot);
-      dot += xor_lanes<32>(dot);
+      dot = add_32(add_16(dot));
       const float u = a.beta[(int64_t)t * a.beta_token + h] * (to_f32(v[(int64_t)t * a.v_token]) - dot);
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
@@ -838,8 +865,7 @@ __global__ __launch_bounds__(64 * kWaves + 256) void k_delta_scan(DeltaArgs a, i
           S[kt][r] = fmaf(to_f32(k[ch]), u, S[kt][r]);
           o = fmaf(to_f32(q[ch]), S[kt][r], o);
         }
-      o += xor_lanes<16>(o);
-      o += xor_lanes<32>(o);
+      o = add_32(add_16(o));
       if (g == 0) out[(int64_t)t * a.out_token] = from_f32<E>(a.scale * o);
     }
   };

@@ -17,11 +17,13 @@ def _rows(t: torch.Tensor, what: str, dtype, shape, device) -> int:
     """Token stride of (tokens, heads[, size]) rows whose tokens are contiguous blocks."""
     if t.dtype != dtype or t.shape != shape or t.device != device:
         raise ValueError(f"delta_rule: {what} must be a {dtype} tensor of shape {tuple(shape)} on {device}")
-    strides, size = t.stride(), 1
-    for i in range(len(shape) - 1, 0, -1):
-        if strides[i] != size and shape[i] > 1:
-            raise ValueError(f"delta_rule: a token's {what} must be contiguous")
-        size *= shape[i]
+    strides = t.stride()
+    if strides[1:] != ((shape[2], 1) if len(shape) == 3 else (1,)):
+        size = 1
+        for n, stride in zip(shape[:0:-1], strides[:0:-1]):  # (a size of 1 may have any stride)
+            if stride != size and n > 1:
+                raise ValueError(f"delta_rule: a token's {what} must be contiguous")
+            size *= n
     return strides[0]
 
 
@@ -59,7 +61,7 @@ def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
         if t is not None:
             require(t, f"delta_rule: {what}", torch.int32, (size,), dev)
     if out is None:
-        out = torch.empty((T, Hv, dv), dtype=q.dtype, device=dev)
+        out = v.new_empty((T, Hv, dv))
     x = DeltaRows(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), out.data_ptr(),
                   _rows(q, "q", q.dtype, (T, Hk, dk), dev), _rows(k, "k", q.dtype, (T, Hk, dk), dev),
                   _rows(v, "v", q.dtype, (T, Hv, dv), dev),
@@ -68,8 +70,8 @@ def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     cfg = _config(q, v, g, scale)
     require_device(q, "delta_rule")
     need = _lib.lib().exl3_delta_workspace_size(C.byref(cfg), T, n)
-    if ws is None or ws.numel() < need:
+    if need and (ws is None or ws.numel() < need):
         ws = _workspace(need, dev)
     call("exl3_delta_rule", C.byref(cfg), C.byref(x), T, _ptr(starts), n, state.data_ptr(), state.shape[0],
-         _ptr(slots), _ptr(dst), ws.data_ptr(), ws.numel(), stream_on(dev))
+         _ptr(slots), _ptr(dst), _ptr(ws), 0 if ws is None else ws.numel(), stream_on(dev))
     return out

@@ -73,10 +73,10 @@ def head_norm(q: torch.Tensor, k: torch.Tensor | None = None, *, mode: str = "rm
         rotate = 2 * inv_freq.numel()
         if rotate > d:
             raise ValueError("head_norm: inv_freq has more than head_dim / 2 frequencies")
-    q_out = q.new_empty(q.shape) if q_out is None else q_out
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else q_out
     sides = [_side("q", q, q_weight, q_out, q.dtype, q.device)]
     if k is not None:
-        k_out = k.new_empty(k.shape) if k_out is None else k_out
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if k_out is None else k_out
         sides.append(_side("k", k, k_weight, k_out, q.dtype, q.device))
     require_device(q, "head_norm")
     cfg = HeadNormConfig(ST_DTYPE[q.dtype], MODES[mode], d, rotate, int(interleaved), eps)
