@@ -690,7 +690,7 @@ __global__ __launch_bounds__(256, 4) void k_delta_chunk(DeltaArgs a) {
 // there (and its values), in the other of two buffers, and load the one after it: the
 // multiplying waves wait for no load, and their stores are never waited for.
 template <typename E, int DK, bool kChannel, int kWaves>
-__global__ __launch_bounds__(64 * kWaves + 256) void k_delta_scan(DeltaArgs a, int parts) {
+__global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
   constexpr int N = DK / 64, KT = DK / 16;
   using St = Stage<E, DK, kWaves>;
   __shared__ St stage[2];
@@ -709,8 +709,12 @@ __global__ __launch_bounds__(64 * kWaves + 256) void k_delta_scan(DeltaArgs a, i
   const ChunkMats *mats = a.chunks + (size_t)first_chunk(s, seq) * a.heads_v + h;
 
   if (wave >= kWaves) {
+    // With two multiplying waves (on the first two SIMDs) the preparing ones share the other two,
+    // two on each, and the waves that would share with the multiplying ones end here.
+    const int helper = kWaves == 2 ? wave % 2 + wave / 4 * 2 : wave - kWaves;
+    if (kWaves == 2 && wave / 2 == 2) return;
     // lane: channels ch .. of tokens 8 g ..
-    const int part = tid - 64 * kWaves, ch = part / 64 * (DK / 4) + m * N;
+    const int part = 64 * helper + lane, ch = part / 64 * (DK / 4) + m * N;
     RawSlice<E, DK, kChannel> raw;
     u32x4 mat[2];
     int fine[2];
@@ -1103,7 +1107,7 @@ exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows 
           constexpr int kWaves = decltype(waves)::value;
           const int parts = (cfg->dv / kCols + kWaves - 1) / kWaves;
           const unsigned blocks = (unsigned)((cfg->heads_v * n_seq + 7) / 8 * 8 * parts);
-          k_delta_scan<E, DK, kChannel, kWaves><<<blocks, 64 * kWaves + 256, 0, st>>>(a, parts);
+          k_delta_scan<E, DK, kChannel, kWaves><<<blocks, 512, 0, st>>>(a, parts);
         };
         if ((cfg->dv / kCols + 1) / 2 * (int64_t)cfg->heads_v * n_seq <= 256) scan(std::integral_constant<int, 2>{});
         else scan(std::integral_constant<int, 4>{});
