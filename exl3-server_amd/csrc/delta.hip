@@ -45,6 +45,7 @@ struct DeltaArgs {
   int64_t n_slots;
   const int32_t *src, *dst;
   ChunkMats *chunks;  // (chunk ids, heads_v)
+  bool words;         // q's and k's rows begin at 4-byte addresses
 };
 
 struct Seq {
@@ -260,7 +261,26 @@ struct RawSlice {
     const char *gb = chunk_rows<float>(a.g, a.g_token, t0, kChannel ? (int64_t)h * DK : h);
     const uint32_t ks = (uint32_t)a.k_token * 2, qs = (uint32_t)a.q_token * 2, gs = (uint32_t)a.g_token * 4;
     const uint32_t c2 = ch * 2, c4 = kChannel ? ch * 4 : 0;
-    if (n >= kC) {
+    if (a.words) {
+      // rows at 4-byte addresses: what lies behind the last one reads as zeros (a decay of 1)
+      auto rows = [&](const char *p, uint32_t stride, uint32_t bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc((void *)p, (short)0, (int)(uniform(min(n, kC) - 1) * stride + bytes), 0x00020000);
+      };
+      const __amdgpu_buffer_rsrc_t kr = rows(kb, ks, DK * 2), qr = rows(qb, qs, DK * 2), gr = rows(gb, gs, kChannel ? DK * 4 : 4);
+      const int ko = tok * ks + c2, qo = tok * qs + c2, go = tok * gs + c4;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (N == 2) {
+          k[i] = bitcast<EN>((uint32_t)__builtin_amdgcn_raw_buffer_load_b32(kr, ko + i * ks, 0, 0));
+          q[i] = bitcast<EN>((uint32_t)__builtin_amdgcn_raw_buffer_load_b32(qr, qo + i * qs, 0, 0));
+        } else {
+          k[i] = bitcast<EN>((uint16_t)__builtin_amdgcn_raw_buffer_load_b16(kr, ko + i * ks, 0, 0));
+          q[i] = bitcast<EN>((uint16_t)__builtin_amdgcn_raw_buffer_load_b16(qr, qo + i * qs, 0, 0));
+        }
+        if constexpr (G == 2) g[i] = bitcast<GN>(__builtin_amdgcn_raw_buffer_load_b64(gr, go + i * gs, 0, 0));
+        else g[i] = bitcast<GN>(__builtin_amdgcn_raw_buffer_load_b32(gr, go + i * gs, 0, 0));
+      }
+    } else if (n >= kC) {
       const uint32_t ko = tok * ks + c2, qo = tok * qs + c2, go = tok * gs + c4;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -356,16 +376,25 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// Where value `col` of an LDS row of left operands lies: the rows' 16-byte pieces are turned
+// among themselves so that the 16-byte reads of 16 rows (and the reads of the lane groups beside
+// them) meet no bank twice, without padding. Rows of DK channels, and of 32 tokens.
+template <int DK>
+__device__ __forceinline__ constexpr int channel_at(int row, int col) {
+  return col ^ (DK == 128 ? row & 15 : row >> 1 & 7) * 8;
+}
+__device__ __forceinline__ constexpr int token_at(int row, int col) { return col ^ (-(row >> 2) & 3) * 8; }
+
 // One chunk's left operands in LDS, rows in operand order, and the decay over the chunk.
 template <typename E, int DK, int kWaves>
 struct alignas(16) Stage {
   static constexpr int kCol = kWaves * kCols + 8;
-  static constexpr int kRow = DK + 8, kTok = kC + 8;  // f16; 16-byte reads of 16 rows meet no bank twice
-  f16 pk[2][kC][kRow], pq[2][kC][kRow];  // P K, P Q: hi, lo
-  f16 pe[2][DK][kTok];                   // (P_C / P K)^T
-  f16 mat[4][kC][kTok];                  // T hi, T lo, B hi, B lo
+  f16 pk[2][kC][DK], pq[2][kC][DK];  // P K, P Q: hi, lo (channel_at)
+  f16 pe[2][DK][kC];                 // (P_C / P K)^T (token_at)
+  f16 mat[4][kC][kC];                // T hi, T lo, B hi, B lo (token_at)
   E v[kC][kCol];
   float decay[DK];
+  uint32_t v_bad[4];  // by preparing wave: the column blocks in which a value is infinite or NaN
   int fine;
 };
 
@@ -478,9 +507,9 @@ __device__ __forceinline__ void wave_sums8(float (&v)[8]) {
 // and 1 multiply A's and B's tiles of h = 1, 4, 16, waves 2 and 3 those of 2 and 8.
 template <typename E, int DK, bool kChannel>
 __global__ __launch_bounds__(256, 4) void k_delta_chunk(DeltaArgs a) {
-  constexpr int N = DK / 64, kRow = DK + 8;
+  constexpr int N = DK / 64;
   struct Operands {
-    f16 left_k[2][16][kRow], left_q[2][16][kRow], right[2][16][kRow];  // hi, lo, times 2^6
+    f16 left_k[2][16][DK], left_q[2][16][DK], right[2][16][DK];  // hi, lo, times 2^6 (channel_at)
   };
   struct Results {
     float A[kC][kC + kPad], B[kC][kC + kPad];
@@ -547,11 +576,13 @@ __global__ __launch_bounds__(256, 4) void k_delta_chunk(DeltaArgs a) {
     const int hh = 1 << level;
     if (level) __syncthreads();  // the last tile's operands are read
     auto put_left = [&](int row, int i) {
-      put_split<N>(&lds.in.left_k[0][row][lane * N], &lds.in.left_k[1][row][lane * N], x.k[i], x.P[i]);
-      put_split<N>(&lds.in.left_q[0][row][lane * N], &lds.in.left_q[1][row][lane * N], x.q[i], x.P[i]);
+      const int at = channel_at<DK>(row, lane * N);
+      put_split<N>(&lds.in.left_k[0][row][at], &lds.in.left_k[1][row][at], x.k[i], x.P[i]);
+      put_split<N>(&lds.in.left_q[0][row][at], &lds.in.left_q[1][row][at], x.q[i], x.P[i]);
     };
     auto put_right = [&](int row, int i) {
-      put_split<N>(&lds.in.right[0][row][lane * N], &lds.in.right[1][row][lane * N], x.k[i], x.X[i]);
+      const int at = channel_at<DK>(row, lane * N);
+      put_split<N>(&lds.in.right[0][row][at], &lds.in.right[1][row][at], x.k[i], x.X[i]);
     };
     if (hh < 8) {
 #pragma unroll
@@ -574,9 +605,9 @@ __global__ __launch_bounds__(256, 4) void k_delta_chunk(DeltaArgs a) {
     if (hh == 4) put<N>(&total[wave][lane * N], x.P[7]);
     __syncthreads();
     if (wave / 2 == level % 2) {
-      auto operand = [&](const f16(&p)[2][16][kRow], int k0) {
-        return Pair{*reinterpret_cast<const f16x8 *>(&p[0][lane % 16][k0 + lane / 16 * 8]),
-                    *reinterpret_cast<const f16x8 *>(&p[1][lane % 16][k0 + lane / 16 * 8])};
+      auto operand = [&](const f16(&p)[2][16][DK], int k0) {
+        const int at = channel_at<DK>(lane % 16, k0 + lane / 16 * 8);
+        return Pair{*reinterpret_cast<const f16x8 *>(&p[0][lane % 16][at]), *reinterpret_cast<const f16x8 *>(&p[1][lane % 16][at])};
       };
       Pair l[DK / 32][1], r[DK / 32];
 #pragma unroll
@@ -767,8 +798,9 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
           k[j] = to_f32((E)raw.k[i][j]);
           q[j] = to_f32((E)raw.q[i][j]);
         }
-        put_split<N>(&st.pk[0][8 * g + i][col], &st.pk[1][8 * g + i][col], k, before);
-        put_split<N>(&st.pq[0][8 * g + i][col], &st.pq[1][8 * g + i][col], q, before);
+        const int row = 8 * g + i, at = channel_at<DK>(row, col);
+        put_split<N>(&st.pk[0][row][at], &st.pk[1][row][at], k, before);
+        put_split<N>(&st.pq[0][row][at], &st.pq[1][row][at], q, before);
       }
 #pragma unroll
       for (int j = 0; j < N; ++j)
@@ -781,16 +813,28 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
             x4[t] = behind[j];
             behind[j] *= d[i + t][j];
           }
-          const int at = in_order(8 * g + i);
+          const int at = token_at(ch + j, in_order(8 * g + i));
           put_split<4>(&st.pe[0][ch + j][at], &st.pe[1][ch + j][at], k4, x4);
         }
       if (g == 0) put<N>(&st.decay[ch], all);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int at = part + 256 * i;  // of 512 pieces of 8 values: 4 matrices of 32 rows of 4
-        *reinterpret_cast<u32x4 *>(&st.mat[at / 128][at / 4 % 32][at % 4 * 8]) = mat[i];
+        *reinterpret_cast<u32x4 *>(&st.mat[at / 128][at / 4 % 32][token_at(at / 4 % 32, at % 4 * 8)]) = mat[i];
       }
       if (part == 0) st.fine = fine[0] && fine[1];
+      // infinities and NaN by their bits
+      const uint16_t inf = bitcast<uint16_t>(from_f32<E>(INFINITY));
+      typedef uint16_t U8 __attribute__((ext_vector_type(8)));
+      const U8 bits = bitcast<U8>(val) & (uint16_t)0x7fff;
+      uint16_t most = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = bits[i] > most ? bits[i] : most;
+      const uint64_t bad = __ballot(most >= inf);
+      uint32_t tiles = 0;
+#pragma unroll
+      for (int t = 0; t < kWaves; ++t) tiles |= bad & ((kPieces == 4 ? 0x3333333333333333ull : 0x0303030303030303ull) << (2 * t)) ? 1u << t : 0u;
+      if (lane == 0) st.v_bad[helper] = tiles;
       if (part / kPieces >= s.last - (s.first + c * kC)) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) val[i] = from_f32<E>(0.0f);
@@ -828,19 +872,11 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
   const E *v = reinterpret_cast<const E *>(a.v) + (int64_t)h * a.dv + col;
   E *out = reinterpret_cast<E *>(a.out) + (int64_t)h * a.dv + col;
 
-  // Whether chunk c may be multiplied, and its values.
-  f32x4 V[2];
+  // Whether chunk c may be multiplied.
   auto fine_chunk = [&](int c) {
     const St &st = stage[c & 1];
-    float z = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        V[i][r] = to_f32(st.v[16 * i + 4 * g + r][wave * kCols + m]);
-        z = fmaf(0.0f, V[i][r], z);
-      }
-    return st.fine && !__any(z != 0.0f);
+    const uint32_t bad = st.v_bad[0] | st.v_bad[1] | st.v_bad[2] | st.v_bad[3];
+    return uniform(st.fine && !(bad >> wave & 1)) != 0;
   };
   // Chunk c token by token in f32, where something in it is infinite, NaN or out of range, so
   // that it reaches no earlier token.
@@ -873,41 +909,61 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
       if (g == 0) out[(int64_t)t * a.out_token] = from_f32<E>(a.scale * o);
     }
   };
+  // The largest of this lane's part of its column.
+  float most_state;
+  auto weigh = [&] {
+    most_state = 0.0f;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) most_state = most_of(S[kt], most_state);
+  };
+  weigh();
   auto multiply = [&](int c) {
     const int t0 = s.first + c * kC, n = s.last - t0;
     const St &st = stage[c & 1];
-    auto left = [&](const f16 *hi, const f16 *lo) {
-      return Pair{*reinterpret_cast<const f16x8 *>(hi + 8 * g), *reinterpret_cast<const f16x8 *>(lo + 8 * g)};
+    auto by_channel = [&](const f16(&p)[2][kC][DK], int i, int u) {
+      const int at = channel_at<DK>(m, 32 * u + 8 * g);
+      return Pair{*reinterpret_cast<const f16x8 *>(&p[0][16 * i + m][at]), *reinterpret_cast<const f16x8 *>(&p[1][16 * i + m][at])};
+    };
+    auto by_tokens = [&](const f16 *hi, const f16 *lo) {
+      const int at = token_at(m, 8 * g);
+      return Pair{*reinterpret_cast<const f16x8 *>(hi + at), *reinterpret_cast<const f16x8 *>(lo + at)};
     };
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
     constexpr int UT = KT / 2;
-    // left operands are read well before their products
+    // left operands are read well before their products, among the state's splitting
     Pair pk[UT][2], pq[UT][2], right[UT];
+    const ColumnScale ss(most_state);
 #pragma unroll
     for (int u = 0; u < UT; ++u)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) pk[u][i] = left(&st.pk[0][16 * i + m][32 * u], &st.pk[1][16 * i + m][32 * u]);
+      for (int i = 0; i < 2; ++i) pk[u][i] = by_channel(st.pk, i, u);
 #pragma unroll
     for (int u = 0; u < UT; ++u)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) pq[u][i] = left(&st.pq[0][16 * i + m][32 * u], &st.pq[1][16 * i + m][32 * u]);
-    __builtin_amdgcn_sched_barrier(0);
-    float most = 0.0f;
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) most = most_of(S[kt], most);
-    const ColumnScale ss(most);
+      for (int i = 0; i < 2; ++i) pq[u][i] = by_channel(st.pq, i, u);
 #pragma unroll
     for (int u = 0; u < UT; ++u) right[u] = split(S[2 * u], S[2 * u + 1], ss.to);
+#pragma unroll
+    for (int i = 0; i < 8 * UT; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // an LDS read,
+      __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // four vector instructions
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 V[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) V[i][r] = to_f32(st.v[16 * i + 4 * g + r][wave * kCols + m]);
     f32x4 X[2] = {zero, zero}, O[2] = {zero, zero}, W[2] = {zero, zero}, BU[2] = {zero, zero};
     product<UT, 2>(pk, right, X);
     product<UT, 2>(pq, right, O);
     Pair mt[1][2], mb[1][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) mt[0][i] = left(st.mat[0][16 * i + m], st.mat[1][16 * i + m]);
+    for (int i = 0; i < 2; ++i) mt[0][i] = by_tokens(st.mat[0][16 * i + m], st.mat[1][16 * i + m]);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) mb[0][i] = left(st.mat[2][16 * i + m], st.mat[3][16 * i + m]);
+    for (int i = 0; i < 2; ++i) mb[0][i] = by_tokens(st.mat[2][16 * i + m], st.mat[3][16 * i + m]);
     const float cs = ss.back / kScale;
-    most = 0.0f;
+    float most = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -919,7 +975,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
     product<1, 2>(mt, x, W);
     Pair pe[1][KT];
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) pe[0][kt] = left(st.pe[0][16 * kt + m], st.pe[1][16 * kt + m]);
+    for (int kt = 0; kt < KT; ++kt) pe[0][kt] = by_tokens(st.pe[0][16 * kt + m], st.pe[1][16 * kt + m]);
     most = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -941,6 +997,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) S[kt][r] = fmaf(cu, add[kt][r], d[r] * S[kt][r]);
     }
+    weigh();
     char *ob = const_cast<char *>(chunk_rows<E>(a.out, a.out_token, t0, (int64_t)h * a.dv));
     const uint32_t os = (uint32_t)a.out_token * 2, oo = 4 * g * os + col * 2;
     E o[2][4];
@@ -967,6 +1024,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
     for (; c < chunks && fine_chunk(c); ++c, lds_barrier()) multiply(c);
     if (c == chunks) break;
     by_token(c);
+    weigh();
   }
   if (write)
 #pragma unroll
@@ -1092,6 +1150,7 @@ exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows 
   a.src = src;
   a.dst = dst ? dst : src;
   a.chunks = reinterpret_cast<ChunkMats *>(workspace);
+  a.words = (reinterpret_cast<uintptr_t>(x->q) | reinterpret_cast<uintptr_t>(x->k)) % 4 == 0 && (x->q_token | x->k_token) % 2 == 0;
   with_elem16(cfg->dtype, [&](auto e) {
     using E = decltype(e);
     with_form(cfg->dk, cfg->channel_decay != 0, [&](auto dk, auto channel) {
