@@ -8,7 +8,7 @@
 //  k_delta_chunk, k_delta_scan   chunks of C = 32 tokens. With the chunk's first state S0, the
 //    running products P_i = a_1 .. a_i and U the rows u of the rule:
 //      A_ij = k_i . (P_i / P_j) k_j (j < i),  B_ij = q_i . (P_i / P_j) k_j (j <= i)
-//      U = T (V - (P K) S0),  T = (I + diag(beta) A)^-1 diag(beta)
+//      U = T diag(beta) (V - (P K) S0),  T = (I + diag(beta) A)^-1
 //      out = scale ((P Q) S0 + B U),  S <- diag(P_C) S0 + (P_C / P K)^T U
 //    k_delta_chunk computes T and B of every chunk and head side by side; k_delta_scan goes
 //    through a sequence's chunks with its state in registers.
@@ -193,15 +193,17 @@ constexpr int kPad = 4;              // words behind an f32 LDS row: 16-byte rea
 
 // The scan multiplies f16 pairs: x = hi + lo, hi = f16(x), lo = f16(x - hi), 22 bits of x, and
 // three of the four products (lo lo is under 2^-22 of the result). Keys, queries, T and B
-// go in times 2^6, so that the lo of a unit key's values is no subnormal; state columns and
-// the rows between by a power of two that brings the column's largest value to 2^13.
-// A chunk whose values lie outside (|k|, |q|, |T|, |B| under 2^9, decays at most 1) is done
-// token by token in f32.
-constexpr float kScale = 64.0f, kLimit = 512.0f;
+// go in times 2^6, which leaves an error of at most 2^-31 where lo is a subnormal; state columns
+// and the rows between by a power of two that brings the column's largest value to 2^13.
+// A chunk whose values lie outside is done token by token in f32: |k|, |q|, |T|, |B| of 2^9 or
+// more, decays over 1, a key whose largest value is under 2^-8 (2^-31 is 2^-23 of that) or a
+// query's under 2^-16 (2^-15, of a result with 11 bits), unless all its values are 0.
+constexpr float kScale = 64.0f, kLimit = 512.0f, kLeastKey = 0x1p-8f, kLeastQuery = 0x1p-16f;
 // Of one chunk and head, in the workspace: T and B as hi and lo, the columns in operand order,
 // and two marks of a chunk that the scan may multiply.
 struct ChunkMats {
   f16 mat[4][kC][kC];  // T hi, T lo, B hi, B lo
+  float beta[kC];
   int32_t fine[4];     // [0], [1] used
 };
 static_assert(sizeof(ChunkMats) % 16 == 0, "16-byte loads");
@@ -320,22 +322,41 @@ struct Slice {
       }
   }
   // Whether the scan may multiply these values, by their bits: magnitudes order as integers,
-  // infinities and NaN above all others.
+  // infinities and NaN above all others. Called by whole waves that hold whole tokens.
   __device__ __forceinline__ bool fine(const RawSlice<E, DK, kChannel> &x) const {
     typedef uint16_t U __attribute__((ext_vector_type(N)));
-    U most = 0;
+    typedef uint16_t U2 __attribute__((ext_vector_type(2)));
+    U2 most[8];  // of token i's key and query
     uint32_t decay = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      most = __builtin_elementwise_max(most, __builtin_elementwise_max((U)(bitcast<U>(x.k[i]) & (uint16_t)0x7fff),
-                                                                       (U)(bitcast<U>(x.q[i]) & (uint16_t)0x7fff)));
+      const U k = bitcast<U>(x.k[i]) & (uint16_t)0x7fff, q = bitcast<U>(x.q[i]) & (uint16_t)0x7fff;
+      most[i] = U2{k[0], q[0]};
+      if constexpr (N == 2) most[i] = __builtin_elementwise_max(most[i], U2{k[1], q[1]});
 #pragma unroll
       for (int n = 0; n < N; ++n) decay = max(decay, bitcast<uint32_t>(P[i][n]));
     }
-    const uint16_t limit = bitcast<uint16_t>(from_f32<E>(kLimit));
-    bool ok = decay <= 0x3f800000u;  // 1.0f
+    // over the wave: halves and rows exchanged with half of the tokens each, then within 16 lanes
+    auto larger = [](uint32_t a, uint32_t b) { return __builtin_elementwise_max(bitcast<U2>(a), bitcast<U2>(b)); };
 #pragma unroll
-    for (int n = 0; n < N; ++n) ok = ok && most[n] < limit;
+    for (int i = 0; i < 4; ++i) {
+      const auto r = __builtin_amdgcn_permlane32_swap(bitcast<uint32_t>(most[i]), bitcast<uint32_t>(most[i + 4]), false, false);
+      most[i] = larger(r[0], r[1]);
+    }
+    bool ok = decay <= 0x3f800000u;  // 1.0f
+    const uint16_t limit = bitcast<uint16_t>(from_f32<E>(kLimit));
+    const uint16_t key = bitcast<uint16_t>(from_f32<E>(kLeastKey)), query = bitcast<uint16_t>(from_f32<E>(kLeastQuery));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const auto r = __builtin_amdgcn_permlane16_swap(bitcast<uint32_t>(most[i]), bitcast<uint32_t>(most[i + 2]), false, false);
+      uint32_t m = bitcast<uint32_t>(larger(r[0], r[1]));
+      m = bitcast<uint32_t>(larger(m, __builtin_amdgcn_mov_dpp(m, 0xB1, 0xF, 0xF, false)));
+      m = bitcast<uint32_t>(larger(m, __builtin_amdgcn_mov_dpp(m, 0x4E, 0xF, 0xF, false)));
+      m = bitcast<uint32_t>(larger(m, __builtin_amdgcn_mov_dpp(m, 0x141, 0xF, 0xF, false)));
+      m = bitcast<uint32_t>(larger(m, __builtin_amdgcn_mov_dpp(m, 0x140, 0xF, 0xF, false)));
+      const U2 of = bitcast<U2>(m);
+      ok = ok && of[0] < limit && of[1] < limit && (of[0] == 0 || of[0] >= key) && (of[1] == 0 || of[1] >= query);
+    }
     return ok;
   }
   // from blocks of h to blocks of 2 h tokens (h = 1, 2, 4)
@@ -394,6 +415,7 @@ struct alignas(16) Stage {
   f16 mat[4][kC][kC];                // T hi, T lo, B hi, B lo (token_at)
   E v[kC][kCol];
   float decay[DK];
+  float beta[kC];
   uint32_t v_bad[4];  // by preparing wave: the column blocks in which a value is infinite or NaN
   int fine;
 };
@@ -513,7 +535,7 @@ __global__ __launch_bounds__(256, 4) void k_delta_chunk(DeltaArgs a) {
   };
   struct Results {
     float A[kC][kC + kPad], B[kC][kC + kPad];
-    float t00[16][16 + kPad], m11[16][16 + kPad];  // columns
+    float m00[16][16 + kPad], m11[16][16 + kPad];  // columns
     f16 mat[4][kC][kC];                            // as ChunkMats
     int fine[2];
   };
@@ -655,7 +677,6 @@ __global__ __launch_bounds__(256, 4) void k_delta_chunk(DeltaArgs a) {
     // of the second by forward substitution, then -M11 N10 M00 as two small products
     const int col = lane % 16, g = lane / 16, block = g & 1;
     float t[16], most = 0.0f;
-    const float bj = beta[16 * block + col];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float v = 0.0f;
@@ -667,16 +688,15 @@ __global__ __launch_bounds__(256, 4) void k_delta_chunk(DeltaArgs a) {
     if (lane < 32) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float v = t[i] * bj;
-        (block ? lds.out.m11 : lds.out.t00)[col][i] = block ? t[i] : v;
-        most = fmaxf(most, fabsf(v));
-        put_out(0, 16 * block + i, 16 * block + col, v);
+        (block ? lds.out.m11 : lds.out.m00)[col][i] = t[i];
+        most = fmaxf(most, fabsf(t[i]));
+        put_out(0, 16 * block + i, 16 * block + col, t[i]);
       }
     }
     __builtin_amdgcn_wave_barrier();
     f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f}, z = y, m;
     y = mfma4(*reinterpret_cast<const f32x4 *>(&lds.out.A[16 + col][4 * g]),
-              *reinterpret_cast<const f32x4 *>(&lds.out.t00[col][4 * g]), y);
+              *reinterpret_cast<const f32x4 *>(&lds.out.m00[col][4 * g]), y);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       y[r] *= -beta[16 + 4 * g + r];
@@ -711,12 +731,13 @@ __global__ __launch_bounds__(256, 4) void k_delta_chunk(DeltaArgs a) {
   for (int k = 0; k < 2; ++k)
     reinterpret_cast<u32x4 *>(out.mat)[tid + 256 * k] = reinterpret_cast<const u32x4 *>(lds.out.mat)[tid + 256 * k];
   if (tid < 2) out.fine[tid] = lds.out.fine[tid];
+  if (tid < kC) out.beta[tid] = beta[tid];
 }
 
 // A sequence's chunks in turn. The first kWaves waves hold kCols columns of the state each, as the
 // accumulators of DK / 16 tiles: lane l column l % 16, rows 16 kt + 4 (l / 16) + r. As the rows
 // of a result are taken for the k indices of the next product (`in_order`), the state,
-// V - (P K) S0 and U go from result to right operand within the lane; only the left operands,
+// beta (V - (P K) S0) and U go from result to right operand within the lane; only the left operands,
 // which all waves share, pass through LDS. The four waves behind them prepare the next chunk's
 // there (and its values), in the other of two buffers, and load the one after it: the
 // multiplying waves wait for no load, and their stores are never waited for.
@@ -749,6 +770,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
     RawSlice<E, DK, kChannel> raw;
     u32x4 mat[2];
     int fine[2];
+    float beta;
     // 8 values of a row; kPieces such pieces are the workgroup's columns
     typedef E E8 __attribute__((ext_vector_type(8), aligned(2)));
     constexpr int kPieces = kWaves * kCols / 8;
@@ -766,6 +788,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
         mat[i] = reinterpret_cast<const u32x4 *>(in.mat)[part + 256 * i];
       fine[0] = in.fine[0];
       fine[1] = in.fine[1];
+      beta = in.beta[part % kC];
       const uint32_t t = min(part / kPieces, s.last - t0 - 1);
       const char *vb = chunk_rows<E>(a.v, a.v_token, t0, (int64_t)h * a.dv);
       if (has_v) val = *reinterpret_cast<const E8 *>(vb + (t * (uint32_t)a.v_token + v_col) * 2);
@@ -823,6 +846,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
         *reinterpret_cast<u32x4 *>(&st.mat[at / 128][at / 4 % 32][token_at(at / 4 % 32, at % 4 * 8)]) = mat[i];
       }
       if (part == 0) st.fine = fine[0] && fine[1];
+      if (part < kC) st.beta[part] = beta;
       // infinities and NaN by their bits
       const uint16_t inf = bitcast<uint16_t>(from_f32<E>(INFINITY));
       typedef uint16_t U8 __attribute__((ext_vector_type(8)));
@@ -958,6 +982,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
     product<UT, 2>(pk, right, X);
     product<UT, 2>(pq, right, O);
     Pair mt[1][2], mb[1][2];
+    const f32x4 beta[2] = {*reinterpret_cast<const f32x4 *>(&st.beta[4 * g]), *reinterpret_cast<const f32x4 *>(&st.beta[16 + 4 * g])};
 #pragma unroll
     for (int i = 0; i < 2; ++i) mt[0][i] = by_tokens(st.mat[0][16 * i + m], st.mat[1][16 * i + m]);
 #pragma unroll
@@ -967,7 +992,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) X[i][r] = fmaf(-cs, X[i][r], V[i][r]);
+      for (int r = 0; r < 4; ++r) X[i][r] = beta[i][r] * fmaf(-cs, X[i][r], V[i][r]);
       most = most_of(X[i], most);
     }
     const ColumnScale sx(most);

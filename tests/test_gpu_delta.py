@@ -210,3 +210,97 @@ def test_graph_replays_and_repeats(dev, lens):
         got = out.clone()
         call(eager)  # the states carry on from call to call on both sides
         assert torch.equal(got, out) and torch.equal(live, eager), i
+
+
+@pytest.mark.parametrize("Hk,Hv,dv,lens", [(1, 2, 128, [1500]), (8, 8, 256, [300, 1, 77, 200, 64, 33]), (2, 2, 96, [129])], ids=str)
+@pytest.mark.parametrize("channel", [False, True])
+def test_long_sequences(dev, Hk, Hv, dv, lens, channel):
+    # few workgroups (two column blocks each) and many (four)
+    run(dev, lens, Hk, Hv, 128, dv, channel, seed=dv)
+
+
+@pytest.mark.parametrize("dk", [64, 128])
+@pytest.mark.parametrize("lens", [[1, 1, 1], [70, 33]], ids=str)
+def test_rows_at_odd_addresses(dev, dk, lens):
+    # rows of an odd number of values, beginning one value into a buffer: 2-byte addresses
+    T, H = sum(lens), 2
+    x = delta_inputs(12, dev, T, H, H, dk, 64, True, len(lens))
+    starts = starts_of(lens)
+    want, st = x["v"].clone(), x["state"].clone()
+    delta_rule(x["q"], x["k"], x["v"], x["g"], x["beta"], st, starts=ints(starts, dev), out=want)
+
+    def odd(t):
+        n = t[0].numel()
+        buf = torch.zeros(T * (n + 5) + 1, device=dev, dtype=t.dtype)[1:].view(T, n + 5)
+        buf[:, :n] = t.flatten(1)
+        return buf[:, :n].view(t.shape)
+
+    out, st2 = odd(torch.zeros_like(want)), x["state"].clone()
+    delta_rule(odd(x["q"]), odd(x["k"]), odd(x["v"]), odd(x["g"]), odd(x["beta"]), st2, starts=ints(starts, dev), out=out)
+    assert torch.equal(out, want) and torch.equal(st, st2)
+
+
+def test_columns_of_any_scale(dev):
+    # columns are independent and scale exactly by powers of two (bf16, f32): to the bit, also in
+    # the chunks' f16 pairs, whose scale is each column's own
+    x = delta_inputs(13, dev, 100, 2, 2, 128, 64, True, 1, torch.bfloat16)
+    by = torch.tensor([2.0 ** ((c % 5 - 2) * 12) for c in range(64)], device=dev)
+    a, b = x["state"].clone(), x["state"] * by
+    one = delta_rule(x["q"], x["k"], x["v"], x["g"], x["beta"], a)
+    two = delta_rule(x["q"], x["k"], (x["v"].float() * by).to(torch.bfloat16), x["g"], x["beta"], b)
+    assert torch.equal(one.float() * by, two.float()) and torch.equal(a * by, b)
+
+
+def test_values_out_of_the_pairs_range(dev):
+    # keys of 1000 and growing states: chunks that the matrix instructions do not take
+    def large(x):
+        x["k"][:] = (x["k"].float() * 1000).half()
+        x["beta"][:] = 1e-6
+    run(dev, [80], change=large)
+
+    def growing(x):
+        x["g"][:] = 0.005
+    run(dev, [40], change=growing)
+    run(dev, [40], change=growing, channel=False)
+
+    def only_some(x):  # one chunk of three
+        x["k"][40] = (x["k"][40].float() * 700).half()
+        x["beta"][40] = 1e-6
+    run(dev, [96], change=only_some)
+
+
+def test_zero_and_tiny_inputs(dev):
+    def zeros(x):
+        for n in ("q", "k", "v", "state"):
+            x[n][:] = 0
+    x, out, state = run(dev, [50], change=zeros)
+    assert bool((out == 0).all()) and bool((state[1] == 0).all())
+
+    def tiny(x):
+        x["v"][:] = (x["v"].float() * 1e-30).to(x["v"].dtype)
+        x["state"][:] *= 1e-30
+    run(dev, [50], change=tiny, dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("beta,k_scale,q_scale", [(1e-6, 1.0, 1.0), (1.0, 2.0 ** -12, 1.0), (1e-3, 2.0 ** -7, 2.0 ** -13),
+                                                  (0.5, 1.0, 2.0 ** -30)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_small_writes_keep_their_precision(dev, beta, k_scale, q_scale, dtype):
+    # from zeros, nothing forgotten: the state is a sum of 70 small products, so its error is held
+    # to the state itself (not to the values, which are far larger), by check_delta's count of
+    # roundings; small queries give outputs to half a step of their type
+    scale = 2.0 ** 16
+    if dtype == torch.float16 and q_scale < 2.0 ** -20:  # (f16 has no such queries: plain ones, whose results would overflow)
+        q_scale = scale = 1.0
+    x = delta_inputs(14, dev, 70, 1, 1, 128, 64, True, 1, dtype)
+    x["g"][:], x["beta"][:], x["state"][:] = 0.0, beta, 0.0
+    x["k"], x["q"] = (x["k"].float() * k_scale).to(dtype), (x["q"].float() * q_scale).to(dtype)
+    want, new, _, _ = delta64(**x, starts=[0, 70], src=[0], dst=[0], scale=scale)
+    st = x["state"].clone()
+    out = delta_rule(x["q"], x["k"], x["v"], x["g"], x["beta"], st, scale=scale)
+    rel = 4 * math.sqrt(128 + 16) * 2.0 ** -24 * math.sqrt(71)
+    assert float((st.double() - new).norm() / new.norm()) <= rel
+    # f16 results under 2^-14 are subnormals, 2^-24 apart: each off by up to 2^-25, n of them by
+    # sqrt(n) 2^-25 in norm
+    half, tiny = (2.0 ** -11, 2.0 ** -25) if dtype == torch.float16 else (2.0 ** -8, 0.0)
+    assert float((out.double() - want).norm()) <= (half + 2 * rel) * float(want.norm()) + tiny * math.sqrt(out.numel())
