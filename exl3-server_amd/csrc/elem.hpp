@@ -33,13 +33,14 @@ __device__ __forceinline__ void load8(const E *p, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
 }
-template <typename E>
+template <bool kPast = false, typename E>
 __device__ __forceinline__ void store8(E *p, const float (&v)[8]) {
   typedef E vec __attribute__((ext_vector_type(8)));
   vec x;
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = (E)v[i];
-  *reinterpret_cast<vec *>(p) = x;
+  if constexpr (kPast) __builtin_nontemporal_store(x, reinterpret_cast<vec *>(p));  // past the caches
+  else *reinterpret_cast<vec *>(p) = x;
 }
 
 // Whether the bytes [p, p + n) and [q, q + m) meet.

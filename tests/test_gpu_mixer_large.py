@@ -69,3 +69,17 @@ def test_many_rows(dev):
     for at in (0, 1777, 4999):
         a, b = sample_tokens(x[at:at + 1], u[at:at + 1], top_k=int(k[at]), top_p=0.9)
         assert torch.equal(a, ids[at:at + 1]) and torch.equal(b, probs[at:at + 1])
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_many_heads(dev, interleaved):
+    # results larger than the caches take stores of their own: the same bits as in small calls
+    g = gen(5, dev)
+    q, k = normal(g, (1000, 128, 128), torch.float16), normal(g, (1000, 16, 128), torch.float16)
+    pos = torch.arange(1000, device=dev, dtype=torch.int32)
+    inv = 10000.0 ** (-torch.arange(0, 128, 2, device=dev, dtype=torch.float32) / 128)
+    kw = dict(inv_freq=inv, interleaved=interleaved)
+    a, b = head_norm(q, k, positions=pos, **kw)
+    for at in (0, 500, 999):
+        c, d = head_norm(q[at:at + 1], k[at:at + 1], positions=pos[at:at + 1], **kw)
+        assert torch.equal(a[at:at + 1], c) and torch.equal(b[at:at + 1], d)
