@@ -100,7 +100,10 @@ __device__ __forceinline__ f32x4 sum_rows(f32x4 v) {
 }
 
 // A wave holds kCols columns of the state: lane l the columns 4 (l % 4).. and the DK / 16
-// rows from (l / 4) DK / 16.
+// rows from (l / 4) DK / 16, so that a token needs two sums over 16 lanes and no barrier.
+// Bound by the states' traffic for many sequences (64 of 64 heads of 128 x 128: 537 MB read and
+// written in 108 us a call, 5.0 TB/s, a large copy's rate), by latencies for few (one
+// sequence 5.1 us; 8 of 16 heads with 4 tokens each 9.1-10).
 template <typename E, int DK, bool kChannel>
 __global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a) {
   constexpr int R = DK / 16;
@@ -527,6 +530,9 @@ __device__ __forceinline__ void wave_sums8(float (&v)[8]) {
 // both at most 1 for decays that are. The 16 rows with bit h and the 16 without it are one
 // tile of the matrix instruction, of which the pairs of a common block are taken. Waves 0
 // and 1 multiply A's and B's tiles of h = 1, 4, 16, waves 2 and 3 those of 2 and 8.
+// Bound by latencies at four workgroups a CU (the rows' loads are a third of a workgroup's
+// time, the five levels with their barriers another) and then by its vector instructions:
+// 2048 tokens of 64 heads 63 us, of which those alone would take about 30.
 template <typename E, int DK, bool kChannel>
 __global__ __launch_bounds__(256, 4) void k_delta_chunk(DeltaArgs a) {
   constexpr int N = DK / 64;
@@ -741,6 +747,12 @@ __global__ __launch_bounds__(256, 4) void k_delta_chunk(DeltaArgs a) {
 // which all waves share, pass through LDS. The four waves behind them prepare the next chunk's
 // there (and its values), in the other of two buffers, and load the one after it: the
 // multiplying waves wait for no load, and their stores are never waited for.
+// A sequence's chunks depend on each other, so this is bound by the time of one: about 4200
+// cycles, of which 84 matrix instructions are 1350 and the splitting of the state, V and U
+// beside them most of the rest; the preparing waves need as long for some 370 vector
+// instructions each. 2048 tokens of 64 heads: 64 chunks, 144 us. (With f32 matrix
+// instructions and no preparing waves 749 us; with __syncthreads in place of the barriers of
+// LDS alone 371; rows of LDS padded by 16 bytes instead of turned 154.)
 template <typename E, int DK, bool kChannel, int kWaves>
 __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
   constexpr int N = DK / 64, KT = DK / 16;
@@ -1085,7 +1097,9 @@ exl3_status check_config(const exl3_delta_config *c) {
 }
 
 // Whether a call goes in chunks: by the sequences' mean length, as their lengths are on the
-// device.
+// device. Chunks against steps at 8, 16 and 24 tokens each, in us: one sequence of 64 heads 17.7
+// against 11.0, 17.6 / 18.0, 17.8 / 25.0; 16 of them 82 / 53, 83 / 88, 85 / 122; 64 sequences of 8
+// heads 48 / 30, 48 / 49, 51 / 68.
 bool in_chunks(int64_t tokens, int64_t n_seq) { return tokens >= 16 * n_seq; }
 int64_t chunk_ids(int64_t tokens, int64_t n_seq) { return tokens / kC + n_seq; }
 size_t chunk_bytes(const exl3_delta_config *c, int64_t tokens, int64_t n_seq) {
@@ -1185,8 +1199,9 @@ exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows 
       if (need) {
         k_delta_chunk<E, DK, kChannel><<<dim3((unsigned)chunk_ids(tokens, n_seq), (unsigned)cfg->heads_v), 256, 0, st>>>(a);
         // Two column blocks a workgroup where all workgroups then have a CU of their own, else four,
-        // which share the preparation: a 2048-token sequence of 64 heads 171 against 192 us, 7
-        // sequences of up to 1001 tokens of 32 heads 119 against 94 us.
+        // which share the preparation: a 2048-token sequence of 64 heads 169 against 190 us, 7
+        // sequences of up to 1001 tokens of 32 heads 119 against 94 us (both before the
+        // preparing waves moved to SIMDs of their own, which took 17 us off the first).
         auto scan = [&](auto waves) {
           constexpr int kWaves = decltype(waves)::value;
           const int parts = (cfg->dv / kCols + kWaves - 1) / kWaves;
