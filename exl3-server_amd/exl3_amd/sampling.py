@@ -16,7 +16,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
                   ids: torch.Tensor | None = None, probs: torch.Tensor | None = None,
                   ws: torch.Tensor | None = None):
     """(ids (rows) i32, probs (rows) f32): one token for each row of logits (rows, vocab), f16,
-    bf16 or f32, from u (rows) f32 in [0, 1).
+    bf16 or f32 (one row expanded to all of them works: several tokens of one position), from u (rows) f32 in [0, 1).
 
     In a row's order (largest logit first, equal ones by id) the first top_k are kept, of those
     the fewest that hold top_p of their weight, of those the ones with at least min_p times the
@@ -47,6 +47,6 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     need = _lib.lib().exl3_sample_workspace_size(rows, vocab)
     if ws is None or ws.numel() < need:
         ws = _workspace(need, dev)
-    call("exl3_sample", C.byref(cfg), logits.data_ptr(), rows, vocab, max(vocab, logits.stride(0)), u.data_ptr(),
+    call("exl3_sample", C.byref(cfg), logits.data_ptr(), rows, vocab, logits.stride(0) if rows > 1 else vocab, u.data_ptr(),
          ids.data_ptr(), probs.data_ptr(), ws.data_ptr(), ws.numel(), stream_on(dev))
     return ids, probs
