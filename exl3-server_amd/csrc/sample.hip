@@ -627,8 +627,8 @@ exl3_status exl3_sample(const exl3_sample_config *cfg, const void *logits, int64
     return fail(EXL3_ERR_UNSUPPORTED, "exl3_sample: logits must be f16, bf16 or f32");
   if (bad_shape(rows, vocab))
     return fail(EXL3_ERR_INVALID, "exl3_sample: bad shape (at most 65,535 rows of 1 to 524,288 logits)");
-  if ((row_stride && row_stride < vocab) || row_stride < 0 || row_stride > ((int64_t)1 << 40))
-    return fail(EXL3_ERR_INVALID, "exl3_sample: the row stride must be at least the vocabulary, or 0");
+  if (row_stride < vocab || row_stride > ((int64_t)1 << 40))
+    return fail(EXL3_ERR_INVALID, "exl3_sample: the row stride must be at least the vocabulary");
   if (rows == 0) return EXL3_OK;
   if (!logits || !u || !ids) return fail(EXL3_ERR_INVALID, "exl3_sample: null argument");
   const uintptr_t size = cfg->dtype == EXL3_ST_F32 ? 4 : 2;

@@ -16,7 +16,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
                   ids: torch.Tensor | None = None, probs: torch.Tensor | None = None,
                   ws: torch.Tensor | None = None):
     """(ids (rows) i32, probs (rows) f32): one token for each row of logits (rows, vocab), f16,
-    bf16 or f32 (one row expanded to all of them works: several tokens of one position), from u (rows) f32 in [0, 1).
+    bf16 or f32 (rows apart from each other, so an expanded row is refused), from u (rows) f32 in [0, 1).
 
     In a row's order (largest logit first, equal ones by id) the first top_k are kept, of those
     the fewest that hold top_p of their weight, of those the ones with at least min_p times the

@@ -529,7 +529,7 @@ typedef struct {
   const float *min_ps;         /* (rows) or NULL */
 } exl3_sample_config;
 
-/* One token for each row of logits (rows, vocab; row_stride elements from row to row; 0: one row for all) from
+/* One token for each row of logits (rows, vocab; row_stride elements, at least vocab, from row to row) from
  * u[row] in [0, 1). A row is ordered by logit, largest first, equal ones by lower id, with
  * weights w = exp((logit - largest) / temperature). Kept are the first top_k; of those the
  * fewest that hold top_p of their weight; of those the ones with w >= min_p; always the

@@ -106,7 +106,7 @@ def test_sample_refusals():
     assert sample(rows=-1) == sample(rows=65536) == sample(vocab=0) == sample(vocab=2 ** 19 + 1, stride=2 ** 20) == INVALID
     assert sample(stride=99) == sample(logits=0x1001) == sample(u=0x2002) == sample(ids=0x3001) == sample(probs=0x4002) == INVALID
     assert sample(cfg=with_(SAMPLE, top_ks=0x5002)) == sample(cfg=with_(SAMPLE, dtype=2), logits=0x1002) == INVALID
-    assert sample(stride=-1) == sample(stride=-100) == INVALID
+    assert sample(stride=0) == sample(stride=-100) == INVALID
     need = _lib.lib().exl3_sample_workspace_size(2, 100)
     assert need > 0 and _lib.lib().exl3_sample_workspace_size(0, 100) == 0
     assert sample(nbytes=need - 1) == sample(ws=None) == sample(ws=0x100080) == WORKSPACE
