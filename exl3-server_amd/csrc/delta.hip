@@ -70,10 +70,11 @@ __device__ __forceinline__ int64_t slot_of(const int32_t *slots, int i, int64_t 
 // Whether sequence i may write its slot: one that another sequence reads or writes in the
 // same call keeps its old state. Called by every thread of a workgroup.
 __device__ __forceinline__ bool sole_writer(const DeltaArgs &a, int i, int64_t slot) {
+  if (slot < 0) return false;
   bool met = false;
   for (int j = threadIdx.x; j < a.n_seq; j += blockDim.x)
     if (j != i) met |= slot_of(a.src, j, a.n_slots) == slot || slot_of(a.dst, j, a.n_slots) == slot;
-  return !__syncthreads_or(met) && slot >= 0;
+  return !__syncthreads_or(met);
 }
 
 // x + the partner's x, of lane ^ 16 and of lane ^ 32: an exchange holds both, in either order.
@@ -1108,8 +1109,11 @@ size_t chunk_bytes(const exl3_delta_config *c, int64_t tokens, int64_t n_seq) {
 }
 
 bool bad_counts(int64_t tokens, int64_t n_seq) {
-  return tokens < 0 || tokens > ((int64_t)1 << 30) || n_seq < 0 || n_seq > 65535;
+  return tokens < 0 || tokens > ((int64_t)1 << 27) || n_seq < 0 || n_seq > 65535;
 }
+// Heads of all sequences: a launch holds 2^32 threads in a dimension, the scan four workgroups
+// of 512 a head.
+bool too_many(const exl3_delta_config *c, int64_t n_seq) { return c->heads_v * n_seq > (1 << 20); }
 
 }  // namespace
 
@@ -1118,7 +1122,7 @@ using namespace exl3h;
 extern "C" {
 
 size_t exl3_delta_workspace_size(const exl3_delta_config *cfg, int64_t tokens, int64_t n_seq) {
-  if (check_config(cfg) || bad_counts(tokens, n_seq)) return 0;
+  if (check_config(cfg) || bad_counts(tokens, n_seq) || too_many(cfg, n_seq)) return 0;
   return chunk_bytes(cfg, tokens, n_seq);
 }
 
@@ -1128,7 +1132,9 @@ exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows 
   exl3_status rc = check_config(cfg);
   if (rc) return rc;
   if (bad_counts(tokens, n_seq))
-    return fail(EXL3_ERR_INVALID, "exl3_delta_rule: at most 2^30 tokens of at most 65,535 sequences");
+    return fail(EXL3_ERR_INVALID, "exl3_delta_rule: at most 2^27 tokens of at most 65,535 sequences");
+  if (too_many(cfg, n_seq))
+    return fail(EXL3_ERR_INVALID, "exl3_delta_rule: at most 2^20 value heads over all sequences");
   if (n_seq == 0) return EXL3_OK;
   if (!starts && tokens % n_seq)
     return fail(EXL3_ERR_INVALID, "exl3_delta_rule: without starts the tokens must divide into the sequences");
@@ -1164,6 +1170,9 @@ exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows 
     return fail(EXL3_ERR_WORKSPACE, "exl3_delta_rule: workspace too small: need " + std::to_string(need) + " bytes");
   if (need && reinterpret_cast<uintptr_t>(workspace) % 256)
     return fail(EXL3_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  for (int i = 0; i < 7; ++i)
+    if (need && (i < 6 ? spans_meet(workspace, need, rows[i], span(i, i < 4 ? 2 : 4)) : spans_meet(workspace, need, state, state_bytes)))
+      return fail(EXL3_ERR_INVALID, "exl3_delta_rule: the workspace must not overlap rows or state");
   DeltaArgs a = {};
   a.q = x->q;
   a.k = x->k;

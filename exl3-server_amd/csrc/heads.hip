@@ -23,6 +23,8 @@ using namespace exl3e;
 namespace {
 
 constexpr int kMaxHeadDim = 1024;
+constexpr int64_t kMaxSpan = (int64_t)1 << 48;  // elements that a side's tokens or heads span
+constexpr int64_t kMostTokens = 1 << 22;        // of a launch, which holds 2^32 threads in a dimension
 constexpr int kMaxFastDim = 512;  // 64 lanes of 8 values
 constexpr int kThreads = 256;
 constexpr int kEnough = 4096;     // workgroups, 16 a CU: 2048 tokens of 128 heads 33 us, with 2048 workgroups 35, with 16384 36
@@ -36,7 +38,6 @@ struct HeadSide {
 
 struct HeadArgs {
   HeadSide s[2];
-  int64_t tokens;
   int32_t d, R, interleaved;
   float mean, eps;  // mean: 1 / d, or 1 for the L2 norm
   const int32_t *positions;
@@ -225,13 +226,16 @@ extern "C" exl3_status exl3_head_norm(const exl3_head_norm_config *cfg, const ex
   if (tokens < 0 || tokens > ((int64_t)1 << 31) - 1) return fail(EXL3_ERR_INVALID, "exl3_head_norm: bad token count");
   const exl3_head_rows *sides[2] = {q, k};
   HeadArgs a = {};
+  a.R = cfg->rotate_dims;
   int heads = 0;
   for (int i = 0; i < (k ? 2 : 1); ++i) {
     const exl3_head_rows &s = *sides[i];
-    // head counts of a launch's second dimension; strides that 2^48 elements bound cannot overflow
+    // head counts of a launch's second dimension
     if (s.heads < 1 || s.heads > 32767) return fail(EXL3_ERR_INVALID, "exl3_head_norm: heads must be 1..32767");
     for (int64_t v : {s.x_token, s.x_head, s.y_token, s.y_head})
-      if (v < 0 || v > ((int64_t)1 << 31) * 64) return fail(EXL3_ERR_INVALID, "exl3_head_norm: bad stride");
+      if (v < 0 || v > kMaxSpan / 32768) return fail(EXL3_ERR_INVALID, "exl3_head_norm: bad stride");
+    if (tokens && (s.x_token > kMaxSpan / tokens || s.y_token > kMaxSpan / tokens))
+      return fail(EXL3_ERR_INVALID, "exl3_head_norm: bad stride");
     const bool token_major = (s.heads == 1 || s.y_head >= d) && (tokens <= 1 || s.y_token >= (s.heads - 1) * s.y_head + d);
     const bool head_major = (tokens <= 1 || s.y_token >= d) && (s.heads == 1 || s.y_head >= (tokens - 1) * s.y_token + d);
     if (!token_major && !head_major) return fail(EXL3_ERR_INVALID, "exl3_head_norm: output rows overlap each other");
@@ -246,7 +250,7 @@ extern "C" exl3_status exl3_head_norm(const exl3_head_norm_config *cfg, const ex
       return fail(EXL3_ERR_INVALID, "exl3_head_norm: rows and weights must be 2-byte aligned");
     for (int j = 0; j < (k ? 2 : 1); ++j) {
       const HeadSide &o = a.s[j];
-      const bool in_place = i == j && s.x == s.y && s.x_token == s.y_token && s.x_head == s.y_head;
+      const bool in_place = i == j && s.x == s.y && (tokens == 1 || s.x_token == s.y_token) && (s.heads == 1 || s.x_head == s.y_head);
       if (!in_place && rows_meet(s.y, s.y_token, s.y_head, s.heads, o.x, o.x_token, o.x_head, o.heads, tokens, d))
         return fail(EXL3_ERR_INVALID, "exl3_head_norm: an output overlaps an input (in place: the same rows)");
       if (o.w && spans_meet(reinterpret_cast<uintptr_t>(s.y), span_bytes(s, true, tokens, d),
@@ -262,40 +266,55 @@ extern "C" exl3_status exl3_head_norm(const exl3_head_norm_config *cfg, const ex
     if ((reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(inv_freq)) % 4)
       return fail(EXL3_ERR_INVALID, "exl3_head_norm: positions and inv_freq must be 4-byte aligned");
   }
-  a.tokens = tokens;
+  for (int i = 0; i < (k ? 2 : 1) && a.R; ++i) {
+    const uintptr_t y = reinterpret_cast<uintptr_t>(a.s[i].y);
+    const size_t bytes = span_bytes(a.s[i], true, tokens, d);
+    if (spans_meet(y, bytes, reinterpret_cast<uintptr_t>(positions), (size_t)tokens * 4) ||
+        spans_meet(y, bytes, reinterpret_cast<uintptr_t>(inv_freq), (size_t)a.R * 2))
+      return fail(EXL3_ERR_INVALID, "exl3_head_norm: an output overlaps positions or inv_freq");
+  }
   a.d = d;
-  a.R = cfg->rotate_dims;
   a.interleaved = cfg->interleaved != 0;
   a.mean = cfg->mode == EXL3_NORM_L2 ? 1.0f : 1.0f / (float)d;
   a.eps = cfg->eps;
-  a.positions = positions;
   a.inv_freq = inv_freq;
+  // Results that the L2s (8 of 4 MB) would not hold: past them, 2048 tokens of 128 heads of 128
+  // take 33 us and not 42 (a copy of as many bytes: 28).
+  const bool past = tokens * heads * d * 2 > (32 << 20);
+  const HeadSide whole[2] = {a.s[0], a.s[1]};
   with_elem16(cfg->dtype, [&](auto e) {
     using E = decltype(e);
     const hipStream_t st = stream_of(stream);
     // (halves that end inside a lane's 8 values take the general kernel)
     const bool halves_fit = a.interleaved || a.R % 16 == 0;
-    if (d % 8 || d > kMaxFastDim || !halves_fit || !aligned16(a.s[0]) || (k && !aligned16(a.s[1]))) {
-      k_head_norm_any<E><<<dim3((unsigned)tokens, (unsigned)heads), 64, 0, st>>>(a);
-      return;
+    const bool fast = d % 8 == 0 && d <= kMaxFastDim && halves_fit && aligned16(a.s[0]) && (!k || aligned16(a.s[1]));
+    for (int64_t t0 = 0; t0 < tokens; t0 += kMostTokens) {
+      const int64_t n = tokens - t0 < kMostTokens ? tokens - t0 : kMostTokens;
+      a.positions = a.R ? positions + t0 : nullptr;
+      for (int i = 0; i < (k ? 2 : 1); ++i) {
+        a.s[i].x = reinterpret_cast<const E *>(whole[i].x) + t0 * whole[i].x_token;
+        a.s[i].y = reinterpret_cast<E *>(whole[i].y) + t0 * whole[i].y_token;
+      }
+      if (!fast) {
+        k_head_norm_any<E><<<dim3((unsigned)n, (unsigned)heads), 64, 0, st>>>(a);
+        continue;
+      }
+      auto go = [&](auto lanes) {
+        constexpr int kLanes = decltype(lanes)::value, kAtOnce = kThreads / kLanes;
+        // heads of a workgroup: as many as leave enough workgroups
+        const int64_t passes = (heads + kAtOnce - 1) / kAtOnce;
+        int64_t groups = (kEnough + n - 1) / n;
+        groups = groups < passes ? groups : passes;
+        const int per_group = (int)((passes + groups - 1) / groups) * kAtOnce;
+        const dim3 grid((unsigned)n, (unsigned)((heads + per_group - 1) / per_group));
+        if (past) k_head_norm<E, kLanes, true><<<grid, kThreads, 0, st>>>(a, per_group);
+        else k_head_norm<E, kLanes, false><<<grid, kThreads, 0, st>>>(a, per_group);
+      };
+      if (d <= 64) go(std::integral_constant<int, 8>{});
+      else if (d <= 128) go(std::integral_constant<int, 16>{});
+      else if (d <= 256) go(std::integral_constant<int, 32>{});
+      else go(std::integral_constant<int, 64>{});
     }
-    auto go = [&](auto lanes) {
-      constexpr int kLanes = decltype(lanes)::value, kAtOnce = kThreads / kLanes;
-      // heads of a workgroup: as many as leave enough workgroups
-      const int64_t passes = (heads + kAtOnce - 1) / kAtOnce;
-      int64_t groups = (kEnough + tokens - 1) / tokens;
-      groups = groups < passes ? groups : passes;
-      const int per_group = (int)((passes + groups - 1) / groups) * kAtOnce;
-      const dim3 grid((unsigned)tokens, (unsigned)((heads + per_group - 1) / per_group));
-      // Results that the L2s (8 of 4 MB) would not hold: past them, 2048 tokens of 128 heads of 128
-      // take 33 us and not 42 (a copy of as many bytes: 28).
-      if (tokens * heads * d * 2 > (32 << 20)) k_head_norm<E, kLanes, true><<<grid, kThreads, 0, st>>>(a, per_group);
-      else k_head_norm<E, kLanes, false><<<grid, kThreads, 0, st>>>(a, per_group);
-    };
-    if (d <= 64) go(std::integral_constant<int, 8>{});
-    else if (d <= 128) go(std::integral_constant<int, 16>{});
-    else if (d <= 256) go(std::integral_constant<int, 32>{});
-    else go(std::integral_constant<int, 64>{});
   });
   EXL3_LAUNCHED("k_head_norm");
   return EXL3_OK;

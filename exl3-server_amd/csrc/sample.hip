@@ -642,6 +642,16 @@ exl3_status exl3_sample(const exl3_sample_config *cfg, const void *logits, int64
     return fail(EXL3_ERR_WORKSPACE, "exl3_sample: workspace too small: need " + std::to_string(w.total) + " bytes");
   if (reinterpret_cast<uintptr_t>(workspace) % 256)
     return fail(EXL3_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  // outputs and workspace apart from the logits and each other
+  const struct {
+    const void *p;
+    size_t bytes;
+  } parts[5] = {{logits, (size_t)((rows - 1) * row_stride + vocab) * size}, {u, (size_t)rows * 4},
+                {ids, (size_t)rows * 4}, {probs, probs ? (size_t)rows * 4 : 0}, {workspace, w.total}};
+  for (int i = 2; i < 5; ++i)
+    for (int j = 0; j < i; ++j)
+      if (spans_meet(parts[i].p, parts[i].bytes, parts[j].p, parts[j].bytes))
+        return fail(EXL3_ERR_INVALID, "exl3_sample: ids, probs or the workspace overlaps another argument");
   SampleArgs a = {};
   a.logits = logits;
   a.rows = rows;

@@ -9,8 +9,8 @@ import torch
 
 from . import _lib
 from ._lib import DeltaConfig, DeltaRows, call
-from .heads import ST_DTYPE, require, require_device, stream_on
-from .trellis import _ptr, _workspace
+from .heads import ST_DTYPE, require, require_device, scratch, stream_on
+from .trellis import _ptr
 
 
 def _rows(t: torch.Tensor, what: str, dtype, shape, device) -> int:
@@ -70,8 +70,7 @@ def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     cfg = _config(q, v, g, scale)
     require_device(q, "delta_rule")
     need = _lib.lib().exl3_delta_workspace_size(C.byref(cfg), T, n)
-    if need and (ws is None or ws.numel() < need):
-        ws = _workspace(need, dev)
+    ws = scratch(ws, need, dev, "delta_rule")
     call("exl3_delta_rule", C.byref(cfg), C.byref(x), T, _ptr(starts), n, state.data_ptr(), state.shape[0],
          _ptr(slots), _ptr(dst), _ptr(ws), 0 if ws is None else ws.numel(), stream_on(dev))
     return out

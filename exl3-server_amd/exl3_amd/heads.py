@@ -11,7 +11,7 @@ import ctypes as C
 import torch
 
 from ._lib import NORM_L2, NORM_RMS, HeadNormConfig, HeadRows, call
-from .trellis import _stream
+from .trellis import _stream, _workspace
 
 ST_DTYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # exl3_st_dtype
 MODES = {"rms": NORM_RMS, "l2": NORM_L2}
@@ -35,6 +35,13 @@ def require_device(t: torch.Tensor, what: str) -> None:
     """t lives on the current GPU, whose stream and launches a call uses."""
     if t.device.type != "cuda" or t.device.index != torch.cuda.current_device():
         raise ValueError(f"{what}: tensors must be on the current device")
+
+
+def scratch(ws: torch.Tensor | None, need: int, device, what: str) -> torch.Tensor | None:
+    """The caller's workspace where it holds `need` bytes, else one of the allocator's (None for none)."""
+    if ws is not None and (ws.device != device or ws.dtype != torch.uint8 or not ws.is_contiguous()):
+        raise ValueError(f"{what}: ws must be a contiguous uint8 tensor on {device}")
+    return _workspace(need, device) if need and (ws is None or ws.numel() < need) else ws
 
 
 def _side(what, x, w, y, dtype, device):

@@ -8,8 +8,8 @@ import torch
 
 from . import _lib
 from ._lib import SampleConfig, call
-from .heads import ST_DTYPE, require, require_device, stream_on
-from .trellis import _workspace
+from .heads import ST_DTYPE, require, require_device, scratch, stream_on
+from .trellis import _ptr
 
 
 def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
@@ -45,8 +45,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     require(probs, "sample_tokens: probs", torch.float32, (rows,), dev)
     require_device(logits, "sample_tokens")
     need = _lib.lib().exl3_sample_workspace_size(rows, vocab)
-    if ws is None or ws.numel() < need:
-        ws = _workspace(need, dev)
+    ws = scratch(ws, need, dev, "sample_tokens")
     call("exl3_sample", C.byref(cfg), logits.data_ptr(), rows, vocab, logits.stride(0) if rows > 1 else vocab, u.data_ptr(),
-         ids.data_ptr(), probs.data_ptr(), ws.data_ptr(), ws.numel(), stream_on(dev))
+         ids.data_ptr(), probs.data_ptr(), _ptr(ws), 0 if ws is None else ws.numel(), stream_on(dev))
     return ids, probs

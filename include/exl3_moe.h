@@ -465,7 +465,7 @@ typedef struct {
 /* The heads of one side (queries or keys): value i of head h of token t is
  * x[t * x_token + h * x_head + i] (strides in elements, so a slice of a packed qkv row is
  * read in place); y likewise. y may be x itself (same strides); otherwise no output may
- * overlap an input or the other output. */
+ * overlap an input, positions, inv_freq or the other output. */
 typedef struct {
   const void *x;   /* device */
   const void *w;   /* device (head_dim), or NULL: ones */
@@ -491,7 +491,7 @@ typedef struct {
 } exl3_delta_config;
 
 /* Device rows of a call, token strides in elements (a token's heads lie one behind the
- * other). g is the log of the decay (0 or less; -inf clears), beta the write strength. */
+ * other; strides under 2^24). g is the log of the decay (0 or less; -inf clears), beta the write strength. */
 typedef struct {
   const void *q, *k;  /* (tokens, heads_qk, dk) */
   const void *v;      /* (tokens, heads_v, dv) */
@@ -509,7 +509,8 @@ typedef struct {
  * state is (n_slots, heads_v, dk, dv) f32, 16-byte aligned: sequence i starts from slot
  * src[i] and leaves its last state in slot dst[i] (i32 (n_seq), device; src NULL: slot i; dst
  * NULL: as src, in place). A src outside [0, n_slots) starts from zeros, a dst outside is
- * not stored. A slot that more than one sequence of the call names is read but keeps its old
+ * not stored. At most 2^27 tokens, and 2^20 value heads over all sequences (heads_v * n_seq).
+ * A slot that more than one sequence of the call names is read but keeps its old
  * state, so no call's result depends on which sequence came first. */
 size_t exl3_delta_workspace_size(const exl3_delta_config *cfg, int64_t tokens, int64_t n_seq);
 exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows *x, int64_t tokens,
@@ -536,7 +537,8 @@ typedef struct {
  * first. ids[row] is the first of the order whose running weight exceeds u times the kept
  * weight, probs[row] (may be NULL) its share of the kept weight. Logits of -inf or NaN are
  * never taken; a row of nothing else gets id -1 and probability 0. +inf logits share a row
- * evenly. Weights under 2^-45 count as 0. At most 65,535 rows of 524,288. */
+ * evenly. Weights under 2^-45 count as 0. At most 65,535 rows of 524,288; ids, probs
+ * and the workspace lie apart from the rest. */
 size_t exl3_sample_workspace_size(int64_t rows, int64_t vocab);
 exl3_status exl3_sample(const exl3_sample_config *cfg, const void *logits, int64_t rows, int64_t vocab,
                         int64_t row_stride, const float *u, int32_t *ids, float *probs, void *workspace,

@@ -83,3 +83,35 @@ def test_many_heads(dev, interleaved):
     for at in (0, 500, 999):
         c, d = head_norm(q[at:at + 1], k[at:at + 1], positions=pos[at:at + 1], **kw)
         assert torch.equal(a[at:at + 1], c) and torch.equal(b[at:at + 1], d)
+
+
+def test_more_tokens_than_a_launch(dev):
+    # 2^24 + 5 tokens of one head of 8, by both kernels (16-byte rows, and rows behind one value)
+    T, d = 2 ** 24 + 5, 8
+    x = normal(gen(6, dev), (T, 1, d), torch.float16)
+    pos = torch.arange(T, device=dev, dtype=torch.int32)
+    inv = torch.tensor([1.0, 0.5, 0.25, 0.125], device=dev)
+    odd = torch.empty(T * d + 1, device=dev, dtype=torch.float16)[1:].view(T, 1, d)
+    for interleaved, out in ((True, None), (False, None), (True, odd)):
+        got = head_norm(x, positions=pos, inv_freq=inv, interleaved=interleaved, q_out=out)
+        for a, b in ((0, 3), (2 ** 22 - 2, 2 ** 22 + 2), (2 ** 24 - 1, T)):
+            part = torch.empty((b - a) * d + 1, device=dev, dtype=torch.float16)
+            want = head_norm(x[a:b].contiguous(), positions=pos[a:b].contiguous(), inv_freq=inv, interleaved=interleaved,
+                             q_out=part[1:].view(b - a, 1, d) if out is odd else None)
+            assert torch.equal(got[a:b], want)
+
+
+def test_workspaces_and_one_token_in_place(dev):
+    g = gen(7, dev)
+    x, u = normal(g, (3, 500), torch.float16), torch.tensor([0.1, 0.5, 0.9], device=dev)
+    d = delta_inputs(8, dev, 64, 1, 1, 64, 64, False, 1)
+    for ws in (torch.empty(1 << 22, dtype=torch.uint8), torch.empty(1 << 20, device=dev), torch.empty((1 << 23,), device=dev, dtype=torch.uint8)[::2]):
+        with pytest.raises(ValueError, match="ws"):
+            sample_tokens(x, u, ws=ws)
+        with pytest.raises(ValueError, match="ws"):
+            delta_rule(d["q"], d["k"], d["v"], d["g"], d["beta"], d["state"], ws=ws)
+    # one token, whose stride says nothing, in place
+    q = normal(g, (1, 4, 64), torch.float16)
+    want = head_norm(q)
+    other = q.as_strided((1, 4, 64), (7, 64, 1))
+    assert torch.equal(head_norm(q, q_out=other), want) and torch.equal(q, want)

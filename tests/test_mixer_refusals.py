@@ -56,6 +56,10 @@ def test_head_norm_refusals():
     q = with_(Q, x=0x100000, y=0x100000, **packed)
     k = with_(K, x=0x100000 + 1024 - 2, y=0x100000 + 1024 - 2, **packed)
     assert heads(q=q, k=k) == INVALID and b"overlap" in _lib.lib().exl3_last_error()
+    # on the positions and frequencies; spans that 64 bits would not hold
+    assert heads(pos=0x200000) == heads(inv=0x400000 + 8) == INVALID and b"positions" in _lib.lib().exl3_last_error()
+    assert heads(q=with_(Q, x_token=2 ** 36), tokens=2 ** 31 - 1) == heads(q=with_(Q, y_token=2 ** 33), tokens=2 ** 20) == INVALID
+    assert b"stride" in _lib.lib().exl3_last_error()
     assert heads(tokens=0) == _lib.EXL3_OK
 
 
@@ -83,6 +87,12 @@ def test_delta_rule_refusals():
         assert delta(x=with_(ROWS, **bad)) == INVALID, bad
     for bad in (dict(out=0x12000000), dict(out=0x10000000 + 100), dict(v=0x20000000), dict(out=0x20000000 + 64)):
         assert delta(x=with_(ROWS, **bad)) == INVALID and b"overlap" in _lib.lib().exl3_last_error(), bad
+    # what a launch does not hold: tokens, heads of all sequences
+    assert delta(tokens=2 ** 27 + 1) == delta(tokens=2 ** 20, cfg=with_(DELTA, heads_v=32), n=32769) == INVALID
+    assert b"value heads" in _lib.lib().exl3_last_error()
+    # the workspace on rows or the state
+    for ws in (0x10000000, 0x13000000, 0x15000000 + 0x100, 0x20000000):
+        assert delta(ws=ws) == INVALID and b"workspace" in _lib.lib().exl3_last_error(), hex(ws)
     assert delta(n=0) == _lib.EXL3_OK
     size = _lib.lib().exl3_delta_workspace_size
     assert size(C.byref(with_(DELTA, dk=32)), 64, 2) == 0
@@ -109,6 +119,9 @@ def test_sample_refusals():
     assert sample(stride=0) == sample(stride=-100) == INVALID
     need = _lib.lib().exl3_sample_workspace_size(2, 100)
     assert need > 0 and _lib.lib().exl3_sample_workspace_size(0, 100) == 0
+    for bad in (dict(ids=0x1000), dict(ids=0x2004), dict(probs=0x3004), dict(ids=0x100100), dict(ws=0x1000), dict(logits=0x100000 - 4),
+                dict(probs=0x1000 + 396)):
+        assert sample(**bad) == INVALID and b"overlap" in _lib.lib().exl3_last_error(), bad
     assert sample(nbytes=need - 1) == sample(ws=None) == sample(ws=0x100080) == WORKSPACE
     assert sample(rows=0) == _lib.EXL3_OK
 
