@@ -17,6 +17,7 @@
 // of the decays between, which stays exact where a decay is 0 (g = -inf) or tiny.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <string>
 
 #include "elem.hpp"
@@ -45,6 +46,8 @@ struct DeltaArgs {
   int64_t n_slots;
   const int32_t *src, *dst;
   ChunkMats *chunks;  // (chunk ids, heads_v)
+  int32_t chunked;    // sequences of at least so many tokens go in chunks, the others in steps
+  int32_t scanned;    // at most so many sequences go in chunks
   bool words;         // q's and k's rows begin at 4-byte addresses
 };
 
@@ -75,6 +78,30 @@ __device__ __forceinline__ bool sole_writer(const DeltaArgs &a, int i, int64_t s
   for (int j = threadIdx.x; j < a.n_seq; j += blockDim.x)
     if (j != i) met |= slot_of(a.src, j, a.n_slots) == slot || slot_of(a.dst, j, a.n_slots) == slot;
   return !__syncthreads_or(met);
+}
+
+// The j-th sequence that goes in chunks, or -1. Called by every thread of a workgroup of 512.
+__device__ __forceinline__ int nth_chunked(const DeltaArgs &a, int j) {
+  __shared__ int found, count[8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (tid == 0) found = -1;
+  for (int first = 0; first < a.n_seq; first += 512) {
+    const int i = first + tid;
+    const Seq s = seq_of(a, min(i, a.n_seq - 1));
+    const bool own = i < a.n_seq && s.last - s.first >= a.chunked;
+    const uint64_t lanes = __ballot(own);
+    if (lane == 0) count[wave] = __popcll(lanes);
+    __syncthreads();
+    int before = __popcll(lanes & (((uint64_t)1 << lane) - 1)), all = 0;
+    for (int w = 0; w < 8; ++w) {
+      if (w < wave) before += count[w];
+      all += count[w];
+    }
+    if (own && before == j) found = i;
+    j -= all;
+    __syncthreads();
+  }
+  return found;
 }
 
 // x + the partner's x, of lane ^ 16 and of lane ^ 32: an exchange holds both, in either order.
@@ -109,11 +136,12 @@ template <typename E, int DK, bool kChannel>
 __global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a) {
   constexpr int R = DK / 16;
   const int lane = threadIdx.x & 63, seq = blockIdx.z, h = blockIdx.y, hk = h / (a.heads_v / a.heads_qk);
+  const Seq s = seq_of(a, seq);
+  if (s.last - s.first >= a.chunked) return;
   const int64_t from = slot_of(a.src, seq, a.n_slots), to = slot_of(a.dst, seq, a.n_slots);
   const bool write = sole_writer(a, seq, to);
   const int block = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (block * kCols >= a.dv) return;
-  const Seq s = seq_of(a, seq);
   const int row = lane / 4 * R, col = block * kCols + lane % 4 * 4;
   const size_t head = (size_t)DK * a.dv, at = h * head + (size_t)row * a.dv + col;
   f32x4 S[R];
@@ -531,9 +559,9 @@ __device__ __forceinline__ void wave_sums8(float (&v)[8]) {
 // both at most 1 for decays that are. The 16 rows with bit h and the 16 without it are one
 // tile of the matrix instruction, of which the pairs of a common block are taken. Waves 0
 // and 1 multiply A's and B's tiles of h = 1, 4, 16, waves 2 and 3 those of 2 and 8.
-// Bound by latencies at four workgroups a CU (the rows' loads are a third of a workgroup's
-// time, the five levels with their barriers another) and then by its vector instructions:
-// 2048 tokens of 64 heads 63 us, of which those alone would take about 30.
+// Bound by latencies (its loads, and five levels with a barrier each) at four workgroups a CU:
+// 2048 tokens of 64 heads 63-68 us, where its 1.84e7 vector instructions alone would take
+// about 30. At five workgroups a CU, with the registers that leaves, 98 against 64 us.
 template <typename E, int DK, bool kChannel>
 __global__ __launch_bounds__(256, 4) void k_delta_chunk(DeltaArgs a) {
   constexpr int N = DK / 64;
@@ -570,7 +598,7 @@ __global__ __launch_bounds__(256, 4) void k_delta_chunk(DeltaArgs a) {
   }
   const Seq s = seq_of(a, seq);
   const int chunk = id - first_chunk(s, seq);
-  if (chunk < 0 || chunk >= chunks_of(s)) return;
+  if (chunk < 0 || chunk >= chunks_of(s) || s.last - s.first < a.chunked) return;
   const int t0 = uniform(s.first + chunk * kC), n = uniform(s.last) - t0;
   RawSlice<E, DK, kChannel> raw;
   raw.load(a, t0, n, h, h / (a.heads_v / a.heads_qk), 8 * wave, lane * N);
@@ -751,9 +779,10 @@ __global__ __launch_bounds__(256, 4) void k_delta_chunk(DeltaArgs a) {
 // A sequence's chunks depend on each other, so this is bound by the time of one: about 4200
 // cycles, of which 84 matrix instructions are 1350 and the splitting of the state, V and U
 // beside them most of the rest; the preparing waves need as long for some 370 vector
-// instructions each. 2048 tokens of 64 heads: 64 chunks, 144 us. (With f32 matrix
-// instructions and no preparing waves 749 us; with __syncthreads in place of the barriers of
-// LDS alone 371; rows of LDS padded by 16 bytes instead of turned 154.)
+// instructions each. 2048 tokens of 64 heads: 64 chunks, 144-157 us from run to run.
+// (With f32 matrix instructions and no preparing waves 749 us; with f16 pairs 371; with loads
+// ahead and barriers that wait for LDS alone 193; with the preparing waves on SIMDs of their own
+// 154; with LDS pieces turned, not rows padded, and buffer loads 143.)
 template <typename E, int DK, bool kChannel, int kWaves>
 __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
   constexpr int N = DK / 64, KT = DK / 16;
@@ -763,13 +792,19 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
   // Workgroups go to the 8 XCDs in turn: the `parts` column blocks of one head and sequence
   // to one XCD, whose L2 then reads the rows they share once.
   const int turn = blockIdx.x / 8, part_of = turn % parts, pair = turn / parts * 8 + blockIdx.x % 8;
-  if (pair >= a.heads_v * a.n_seq) return;
-  const int seq = pair / a.heads_v, h = pair % a.heads_v;
+  if (pair >= a.heads_v * a.scanned) return;
+  const int h = pair % a.heads_v;
+  int seq = pair / a.heads_v;
+  if (a.scanned < a.n_seq) {
+    seq = uniform(nth_chunked(a, seq));
+    if (seq < 0) return;
+  }
   const int hk = h / (a.heads_v / a.heads_qk), g = lane / 16, m = lane % 16;
-  const int64_t from = slot_of(a.src, seq, a.n_slots), to = slot_of(a.dst, seq, a.n_slots);
-  const bool write = sole_writer(a, seq, to);
   Seq s = seq_of(a, seq);
   s = Seq{uniform(s.first), uniform(s.last)};
+  if (s.last - s.first < a.chunked) return;
+  const int64_t from = slot_of(a.src, seq, a.n_slots), to = slot_of(a.dst, seq, a.n_slots);
+  const bool write = sole_writer(a, seq, to);
   const int chunks = chunks_of(s);
   const ChunkMats *mats = a.chunks + (size_t)first_chunk(s, seq) * a.heads_v + h;
 
@@ -1097,14 +1132,25 @@ exl3_status check_config(const exl3_delta_config *c) {
   return EXL3_OK;
 }
 
-// Whether a call goes in chunks: by the sequences' mean length, as their lengths are on the
-// device. Chunks against steps at 8, 16 and 24 tokens each, in us: one sequence of 64 heads 17.7
+// Which sequences go in chunks. A sequence does from 16 tokens on: chunks against steps at 8, 16 and 24 tokens each, in us: one sequence of 64 heads 17.7
 // against 11.0, 17.6 / 18.0, 17.8 / 25.0; 16 of them 82 / 53, 83 / 88, 85 / 122; 64 sequences of 8
-// heads 48 / 30, 48 / 49, 51 / 68.
-bool in_chunks(int64_t tokens, int64_t n_seq) { return tokens >= 16 * n_seq; }
+// heads 48 / 30, 48 / 49, 51 / 68. With `starts` the host does not know the lengths, only
+// how many tokens there are: under 64 past one a sequence and under 16 a sequence all go in
+// steps, from 64 a sequence on all in chunks, and between them each by its own length.
+// All steps, all chunks and each by its own, in us for 64 heads: 256 sequences of one token
+// beside one of 2048 3201, 1370, 690; 64 beside one of 128 259, 316, 126; 8 beside one of 512
+// 439, 105, 88; 1 to 1001 tokens 830, 160, 160. The others' launches cost 64 sequences of 4
+// 142 against 136, 16 of them in 16 heads 17 against 14.
+constexpr int kChunked = 16, kFewTokens = 64, kManyTokens = 64;
+enum Form { kSteps, kChunks, kBoth };
+Form form_of(int64_t tokens, int64_t n_seq, bool starts) {
+  if (!starts || n_seq == 1) return tokens >= kChunked * n_seq ? kChunks : kSteps;
+  if (tokens >= kManyTokens * n_seq) return kChunks;
+  return tokens >= kChunked * n_seq || tokens - n_seq >= kFewTokens ? kBoth : kSteps;
+}
 int64_t chunk_ids(int64_t tokens, int64_t n_seq) { return tokens / kC + n_seq; }
-size_t chunk_bytes(const exl3_delta_config *c, int64_t tokens, int64_t n_seq) {
-  return n_seq && in_chunks(tokens, n_seq)
+size_t chunk_bytes(const exl3_delta_config *c, int64_t tokens, int64_t n_seq, bool starts) {
+  return n_seq && form_of(tokens, n_seq, starts) != kSteps
              ? exl3h::align_up((size_t)chunk_ids(tokens, n_seq) * c->heads_v * sizeof(ChunkMats), 256) : 0;
 }
 
@@ -1123,7 +1169,7 @@ extern "C" {
 
 size_t exl3_delta_workspace_size(const exl3_delta_config *cfg, int64_t tokens, int64_t n_seq) {
   if (check_config(cfg) || bad_counts(tokens, n_seq) || too_many(cfg, n_seq)) return 0;
-  return chunk_bytes(cfg, tokens, n_seq);
+  return std::max(chunk_bytes(cfg, tokens, n_seq, true), chunk_bytes(cfg, tokens, n_seq, false));
 }
 
 exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows *x, int64_t tokens,
@@ -1165,7 +1211,8 @@ exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows 
     if ((i != 3 && spans_meet(x->out, span(3, 2), rows[i], span(i, i < 4 ? 2 : 4))) ||
         spans_meet(state, state_bytes, rows[i], span(i, i < 4 ? 2 : 4)))
       return fail(EXL3_ERR_INVALID, "exl3_delta_rule: out and state must not overlap the call's other rows");
-  const size_t need = chunk_bytes(cfg, tokens, n_seq);
+  const Form form = form_of(tokens, n_seq, starts != nullptr);
+  const size_t need = chunk_bytes(cfg, tokens, n_seq, starts != nullptr);
   if (need && (!workspace || workspace_bytes < need))
     return fail(EXL3_ERR_WORKSPACE, "exl3_delta_rule: workspace too small: need " + std::to_string(need) + " bytes");
   if (need && reinterpret_cast<uintptr_t>(workspace) % 256)
@@ -1198,6 +1245,8 @@ exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows 
   a.src = src;
   a.dst = dst ? dst : src;
   a.chunks = reinterpret_cast<ChunkMats *>(workspace);
+  a.chunked = form == kSteps ? INT32_MAX : form == kChunks ? 0 : kChunked;
+  a.scanned = (int32_t)(form == kBoth ? std::min(n_seq, tokens / kChunked) : n_seq);
   a.words = (reinterpret_cast<uintptr_t>(x->q) | reinterpret_cast<uintptr_t>(x->k)) % 4 == 0 && (x->q_token | x->k_token) % 2 == 0;
   with_elem16(cfg->dtype, [&](auto e) {
     using E = decltype(e);
@@ -1205,21 +1254,22 @@ exl3_status exl3_delta_rule(const exl3_delta_config *cfg, const exl3_delta_rows 
       constexpr int DK = decltype(dk)::value;
       constexpr bool kChannel = decltype(channel)::value;
       const hipStream_t st = stream_of(stream);
-      if (need) {
+      if (form != kSteps) {
         k_delta_chunk<E, DK, kChannel><<<dim3((unsigned)chunk_ids(tokens, n_seq), (unsigned)cfg->heads_v), 256, 0, st>>>(a);
         // Two column blocks a workgroup where all workgroups then have a CU of their own, else four,
         // which share the preparation: a 2048-token sequence of 64 heads 169 against 190 us, 7
         // sequences of up to 1001 tokens of 32 heads 119 against 94 us (both before the
-        // preparing waves moved to SIMDs of their own, which took 17 us off the first).
+        // preparing waves moved to SIMDs of their own, which took 16 us off the first).
         auto scan = [&](auto waves) {
           constexpr int kWaves = decltype(waves)::value;
           const int parts = (cfg->dv / kCols + kWaves - 1) / kWaves;
-          const unsigned blocks = (unsigned)((cfg->heads_v * n_seq + 7) / 8 * 8 * parts);
+          const unsigned blocks = (unsigned)(((int64_t)cfg->heads_v * a.scanned + 7) / 8 * 8 * parts);
           k_delta_scan<E, DK, kChannel, kWaves><<<blocks, 512, 0, st>>>(a, parts);
         };
-        if ((cfg->dv / kCols + 1) / 2 * (int64_t)cfg->heads_v * n_seq <= 256) scan(std::integral_constant<int, 2>{});
+        if ((cfg->dv / kCols + 1) / 2 * (int64_t)cfg->heads_v * a.scanned <= 256) scan(std::integral_constant<int, 2>{});
         else scan(std::integral_constant<int, 4>{});
-      } else {
+      }
+      if (form != kChunks) {
         const dim3 grid((unsigned)((cfg->dv / kCols + 3) / 4), (unsigned)cfg->heads_v, (unsigned)n_seq);
         k_delta_step<E, DK, kChannel><<<grid, 256, 0, st>>>(a);
       }

@@ -304,3 +304,59 @@ def test_small_writes_keep_their_precision(dev, beta, k_scale, q_scale, dtype):
     # sqrt(n) 2^-25 in norm
     half, tiny = (2.0 ** -11, 2.0 ** -25) if dtype == torch.float16 else (2.0 ** -8, 0.0)
     assert float((out.double() - want).norm()) <= (half + 2 * rel) * float(want.norm()) + tiny * math.sqrt(out.numel())
+
+
+# single tokens and short sequences beside long ones: each goes by its own length
+MIXED = [[1] * 20 + [100], [100] + [3] * 20, [15, 16, 17, 1, 0, 31, 32, 33, 1, 1], [1] * 9 + [0] + [70] + [1] * 9 + [200], [7] * 12]
+
+
+@pytest.mark.parametrize("lens", MIXED, ids=str)
+@pytest.mark.parametrize("channel", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_mixed_lengths(dev, lens, channel, dtype):
+    run(dev, lens, channel=channel, dtype=dtype, seed=len(lens), first=3, tail=2)
+
+
+@pytest.mark.parametrize("Hk,Hv,dk,dv", [(1, 3, 64, 16), (2, 4, 128, 48), (4, 4, 64, 256)])
+def test_mixed_lengths_of_many_sequences(dev, Hk, Hv, dk, dv):
+    run(dev, [1] * 300 + [40, 2] + [1] * 300 + [90], Hk, Hv, dk, dv, seed=dv, src=list(range(603)), n_slots=603)
+
+
+def test_slots_between_long_and_short_sequences(dev):
+    # sequences 0 and 3 are long: slots that a short one and a long one name, forks, zeros, targets elsewhere
+    lens = [60, 1, 2, 90, 1, 1, 1, 0]
+    run(dev, lens, src=[0, 0, 2, 3, 3, 5, 6, 7], n_slots=8)
+    run(dev, lens, src=[0, 0, 0, 0, 4, 5, 6, 7], dst=[1, 2, 3, 8, 8, 9, 6, 10], n_slots=11)
+    run(dev, lens, src=[1, 0, -1, 99, 4, 5, 6, 7], dst=[0, 1, 2, 3, -1, 9, 8, 7], n_slots=10)
+
+
+def test_mixed_lengths_captured(dev):
+    # the same graph over other lengths of the same total: a sequence goes from steps to chunks and back
+    n, T, H = 12, 200, 2
+    x = delta_inputs(21, dev, T, H, H, 128, 128, True, n)
+    out, ws = torch.empty_like(x["v"]), torch.empty(1 << 22, device=dev, dtype=torch.uint8)
+    all_lens = [[1] * 11 + [189], [100] + [9] * 10 + [10], [17] * 11 + [13], [0] * 10 + [100, 100]]
+    starts, sl = ints(starts_of(all_lens[0]), dev), ints(list(range(n)), dev)
+    call = lambda state: delta_rule(x["q"], x["k"], x["v"], x["g"], x["beta"], state, starts=starts, slots=sl, out=out, ws=ws)  # noqa: E731
+    live, eager = x["state"].clone(), x["state"].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(live)
+    torch.cuda.current_stream().wait_stream(side)
+    live.copy_(eager)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(live)
+    for lens in all_lens:
+        assert sum(lens) == T
+        starts.copy_(ints(starts_of(lens), dev))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        before = eager.clone()
+        call(eager)
+        assert torch.equal(got, out) and torch.equal(live, eager), lens
+        want, new, size, biggest = delta64(x["q"], x["k"], x["v"], x["g"], x["beta"], before, starts_of(lens), list(range(n)),
+                                           list(range(n)), 128 ** -0.5)
+        check_delta(got, live, want, new, size, biggest, starts_of(lens), list(range(n)), 128)
