@@ -52,7 +52,7 @@ constexpr int kThreads = 512;
 constexpr int kGroups = 64, kInGroup = kBins / kGroups;
 constexpr int kList = 1024;           // tokens ordered at once
 constexpr int kMaxSplits = 64, kPerSplit = 8192;  // a lane per split; 13-bit places
-constexpr int kNoBin = 0xffff;
+constexpr float kMost = 3.40282347e38f, kPastBins = (float)(kMaxT * kPerT);
 static_assert(kMaxT * kPerT < kBins, "every weighted token has a bin");
 static_assert(kMaxSplits * kPerSplit >= kMaxVocab, "the splits hold any row");
 static_assert(kPerSplit * 2 <= kBins * 8, "the indices fit where the weights were");
@@ -96,49 +96,45 @@ __device__ __forceinline__ double temperature_of(const SampleArgs &a, int64_t ro
   return (double)(a.temperatures ? a.temperatures[row] : a.temperature);
 }
 
-// A row's tokens against its largest logit m.
+// A row's tokens against its largest logit m (never -inf).
 struct Weigher {
   float m, half_m, per;  // per: bins per half a logit
-  double inv;
+  double top, inv, turn; // m (or the largest finite value), 1 / T, 1 / (T ln 2)
+  double c[10] = {kOne * 7.072578320978871e-09, kOne * 1.0208693139320117e-07, kOne * 1.3215442682805318e-06,
+                  kOne * 1.525265724710113e-05, kOne * 0.00015403530441399083, kOne * 0.0013333558230182842,
+                  kOne * 0.009618129107607343,  kOne * 0.05550410866444765,    kOne * 0.24022650695910097,
+                  kOne * 0.69314718055995};  // of 2^44 2^f, the highest power first
   __device__ __forceinline__ Weigher(float m, double temp)
-      : m(m), half_m(0.5f * m), per((float)(2.0 * kPerT / temp)), inv(1.0 / temp) {}
-  // The token's bin, by f32 alone (it only has to ascend as the logit falls; halved so that no
-  // difference overflows); kNoBin past the last one and for tokens that are never taken.
-  __device__ __forceinline__ int bin(float x) const {
-    if (x == m) return x > -INFINITY ? 0 : kNoBin;  // also +inf
-    const float b = (half_m - 0.5f * x) * per;
-    return b < (float)(kMaxT * kPerT) ? (int)b : kNoBin;  // (no for NaN)
+      : m(m), half_m(0.5f * m), per((float)(2.0 * kPerT / temp)), top(finite(m)), inv(1.0 / temp),
+        turn(1.4426950408889634074 * (1.0 / temp)) {
+    // in scalar registers: from vector ones each would be copied for every value (a fused
+    // multiply-add overwrites its addend there)
+#pragma unroll
+    for (int i = 0; i < 10; ++i) asm("" : "+s"(c[i]));
   }
-  // t, or one past kMaxT for a token that is never taken.
-  __device__ __forceinline__ double t(float x) const {
-    if (!(x > -INFINITY)) return 1e300;
-    if (x == m) return 0.0;  // also +inf
-    const double d = ((double)m - (double)x) * inv;
-    return d < 1e300 ? d : 1e300;
+  static __device__ __forceinline__ double finite(float x) { return (double)__builtin_amdgcn_fmed3f(x, -INFINITY, kMost); }
+  // The token's bin as a number, by f32 alone (it only has to ascend as the logit falls; halved so
+  // that no difference overflows); not under kPastBins for tokens that are never taken.
+  __device__ __forceinline__ float place(float x) const {
+    const float b = fmaf(-0.5f, x, half_m) * per;
+    return x == m ? 0.0f : b;  // (also +inf)
   }
-  // exp(-t) 2^44 (0 from 40 on): -t = (n + f) ln 2, the series of e^(f ln 2) up to the 11th power
-  // (off by 7e-15 of itself).
-  static __device__ __forceinline__ double weight(double t) {
-    if (t > 40.0) return 0.0;
-    const double y = t * -1.4426950408889634074, n = rint(y), r = (y - n) * 0.69314718055994530942;
-    double p = 2.5052108385441719e-8;
-    p = fma(p, r, 2.7557319223985891e-7);
-    p = fma(p, r, 2.7557319223985893e-6);
-    p = fma(p, r, 2.4801587301587302e-5);
-    p = fma(p, r, 1.9841269841269841e-4);
-    p = fma(p, r, 1.3888888888888889e-3);
-    p = fma(p, r, 8.3333333333333333e-3);
-    p = fma(p, r, 4.1666666666666667e-2);
-    p = fma(p, r, 0.16666666666666667);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    return ldexp(p, (int)n + 44);
+  // exp(-t) 2^44 of a token that has a bin: 2^y = 2^n 2^f with f in [-1/2, 1/2], the latter by the
+  // polynomial of degree 10 through 11 Chebyshev points (off by 5e-16 of itself; exact at 0).
+  __device__ __forceinline__ double weight(float x) const {
+    const double y = (finite(x) - top) * turn, n = rint(y), f = y - n;
+    double p = c[0];
+#pragma unroll
+    for (int i = 1; i < 10; ++i) p = fma(p, f, c[i]);
+    p = fma(p, f, kOne);
+    return ldexp(p, (int)n);
   }
   // To the nearest integer: the sum's low bits are it.
   static __device__ __forceinline__ u64 fixed(double w) {
     return bitcast<u64>(w + 4503599627370496.0) & 0x000fffffffffffffull;
   }
+  // exp(-t).
+  __device__ __forceinline__ double share(float x) const { return exp((finite(x) - top) * inv); }
 };
 
 // f(index, value) for the values [first, last) of a row, by `step` threads of which this is
@@ -215,17 +211,18 @@ __global__ __launch_bounds__(kThreads) void k_sample_hist(SampleArgs a) {
   __syncthreads();
   const Weigher W(of_key((uint32_t)(best >> 32)), temp);
   const double least = kOne * (double)(a.min_ps ? a.min_ps[row] : a.min_p);
+  const bool weigh_above = least > 0.0;
   const int first = min(a.vocab, (int)blockIdx.x * a.per_split), last = min(a.vocab, first + a.per_split);
   const E *x = reinterpret_cast<const E *>(a.logits) + row * a.stride;
   u64 above = 0;
   each_value<E, 2>(x, first, last, tid, kThreads, [&](int, float v) {
-    const int b = W.bin(v);
-    if (b == kNoBin) return;
-    const double w = W.weight(W.t(v));
+    const float b = W.place(v);
+    if (!(b < kPastBins)) return;  // (so for NaN)
+    const double w = W.weight(v);
     const u64 f = W.fixed(w);
-    atomicAdd(&count[b], 1u);
-    atomicAdd(&mass[b], f);
-    if (!(w < least)) above += f;
+    atomicAdd(&count[(int)b], 1u);
+    atomicAdd(&mass[(int)b], f);
+    if (weigh_above) above += w < least ? 0 : f;
   });
   above = wave_reduce(above, [](u64 p, u64 q) { return p + q; });
   if (lane == 0) red[wave] = above;
@@ -276,8 +273,8 @@ __global__ __launch_bounds__(kThreads) void k_sample_hist(SampleArgs a) {
   // taken from the logits again, which costs less than the LDS to keep them (3 workgroups a CU)
   uint16_t *ordered = reinterpret_cast<uint16_t *>(mass);
   each_value<E, 2>(x, first, last, tid, kThreads, [&](int i, float v) {
-    const int b = W.bin(v);
-    if (b != kNoBin) ordered[atomicAdd(&count[b], 1u)] = (uint16_t)(i - first);
+    const float b = W.place(v);
+    if (b < kPastBins) ordered[atomicAdd(&count[(int)b], 1u)] = (uint16_t)(i - first);
   });
   __syncthreads();
   uint32_t all = 0;
@@ -369,7 +366,7 @@ struct Pick {
     const uint32_t at = s.begin[k] + j - (k ? s.upto[k - 1] : 0u);
     return k * a.per_split + a.order[(row * a.splits + k) * a.per_split + at];
   }
-  __device__ __forceinline__ u64 mass_of(float v) const { return W.fixed(W.weight(W.t(v))); }
+  __device__ __forceinline__ u64 mass_of(float v) const { return W.fixed(W.weight(v)); }
 
   // The first token of the order where `u` is met, or the last of all where none is. Called
   // by the whole workgroup, and the same for all of it.
@@ -530,6 +527,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_pick(SampleArgs a) {
   const double temp = temperature_of(a, r);
   const int32_t top_k = a.top_ks ? a.top_ks[r] : a.top_k;
   const float top_p = a.top_ps ? a.top_ps[r] : a.top_p;
+  const float min_p = a.min_ps ? a.min_ps[r] : a.min_p;
   const float u = a.u[r];
   u64 m[kMaxSplits * 64 / kThreads];
   uint32_t c[kMaxSplits * 64 / kThreads];
@@ -555,16 +553,18 @@ __global__ __launch_bounds__(kThreads) void k_sample_pick(SampleArgs a) {
   u64 kept = pick.weight();
   if (top_k > 0 && (uint32_t)top_k < pick.tokens()) kept = pick.find(Until{Until::kCount, (uint32_t)top_k, 0.0}).mass;
   if (top_p < 1.0f) kept = pick.find(Until{Until::kAtLeast, 0, (double)top_p * (double)kept}).mass;
-  above = wave_reduce(above, [](u64 p, u64 q) { return p + q; });
-  const u64 first = (u64)kOne;
-  above = above < first ? first : above;
-  kept = above < kept ? above : kept;
+  if (min_p > 0.0f) {
+    above = wave_reduce(above, [](u64 p, u64 q) { return p + q; });
+    const u64 first = (u64)kOne;
+    above = above < first ? first : above;
+    kept = above < kept ? above : kept;
+  }
   // the last kept token where u is 1 or more (or rounding would pass it), the first where u is negative or NaN
   const double goal = (u > 0.0f ? (double)u : 0.0) * (double)kept;
   const Found f = pick.find(goal < (double)kept ? Until{Until::kMore, 0, goal} : Until{Until::kAtLeast, 0, (double)kept});
   if (tid == 0) {
     a.ids[r] = rank_index(f.rank);
-    if (a.probs) a.probs[r] = (float)(exp(-pick.W.t(of_key(rank_key(f.rank)))) / ((double)kept / kOne));
+    if (a.probs) a.probs[r] = (float)(pick.W.share(of_key(rank_key(f.rank))) / ((double)kept / kOne));
   }
 }
 
