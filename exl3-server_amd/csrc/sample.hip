@@ -22,9 +22,9 @@
 //                 of the splits' index lists, and their order; only those tokens' logits are
 //                 read again. A bin with more tokens than the list holds is narrowed by their
 //                 logits' and indices' bits, 11 at a time.
-// Bound by f64 arithmetic and LDS atomics in the histogram for many tokens (64 rows of 154,880 in
-// f32: 8 + 32 + 15 us, where reading them once takes 8), and by the third kernel's chain of
-// dependent loads for few rows (one row: 3 + 8 + 14 us; the groups, a bin's tokens and their
+// Bound by the histogram's vector instructions for many tokens (64 rows of 154,880 in f32: 8 + 24 +
+// 14 us, where reading them once takes 8; its 9.5e6 instructions are about 15 of the 24), and by
+// the third kernel's chain of dependent loads for few rows (one row: 3 + 7 + 14 us; the groups, a bin's tokens and their
 // logits are three of them for each end). Before the index lists, with the row gathered and
 // sorted for each end, one row took 41 us and 8 rows 70.
 #include <hip/hip_runtime.h>
@@ -51,11 +51,11 @@ constexpr double kOne = 17592186044416.0;  // 2^44
 constexpr int kThreads = 512;
 constexpr int kGroups = 64, kInGroup = kBins / kGroups;
 constexpr int kList = 1024;           // tokens ordered at once
-constexpr int kMaxSplits = 64, kPerSplit = 8192;  // a lane per split; 13-bit places
+constexpr int kMaxSplits = 64, kPerSplit = 12288;  // a lane per split; 16-bit places
 constexpr float kMost = 3.40282347e38f, kPastBins = (float)(kMaxT * kPerT);
 static_assert(kMaxT * kPerT < kBins, "every weighted token has a bin");
+constexpr int kMassWords = kPerSplit / 4 > kBins ? kPerSplit / 4 : kBins;
 static_assert(kMaxSplits * kPerSplit >= kMaxVocab, "the splits hold any row");
-static_assert(kPerSplit * 2 <= kBins * 8, "the indices fit where the weights were");
 static_assert(kThreads * 4 == kBins && kInGroup == 32, "four bins a thread, eight threads a group");
 
 typedef unsigned long long u64;
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_max(SampleArgs a) {
 
 template <typename E>
 __global__ __launch_bounds__(kThreads) void k_sample_hist(SampleArgs a) {
-  __shared__ u64 mass[kBins];
+  __shared__ u64 mass[kMassWords];  // then the ordered indices
   __shared__ uint32_t count[kBins];
   __shared__ u64 red[kThreads / 64];
   __shared__ uint32_t wave_count[kThreads / 64];
@@ -568,13 +568,15 @@ __global__ __launch_bounds__(kThreads) void k_sample_pick(SampleArgs a) {
   }
 }
 
-// The splits of a row: of at most kPerSplit tokens, more of them where there are few rows.
+// The splits of a row: of at most kPerSplit tokens, more of them where there are few rows, and
+// where it can be no more workgroups than the 1024 that the card holds at once (4 a CU): 200
+// rows of 32,003 in 5 splits 33.0 us and in 6 35.6, 64 rows of 154,880 in 16 44.9 and in 19 46.5.
 struct Split {
   int splits, per_split;
 };
 Split split_of(int64_t rows, int64_t vocab) {
   const int64_t least = (vocab + kPerSplit - 1) / kPerSplit, most = (vocab + 2047) / 2048;
-  int64_t n = (1024 + rows - 1) / rows;
+  int64_t n = 1024 / rows;
   n = n > most ? most : n;
   n = n < least ? least : n;
   n = n > kMaxSplits ? kMaxSplits : n;
