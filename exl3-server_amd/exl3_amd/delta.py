@@ -48,7 +48,7 @@ def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     than one sequence keeps its old state. scale: 1 / sqrt(dk) unless given."""
     if q.dim() != 3 or v.dim() != 3 or g.dim() not in (2, 3) or q.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError("delta_rule: q and v must be (tokens, heads, size) in float16 or bfloat16, g (tokens, heads[, dk])")
-    dev, (T, Hk, dk), (_, Hv, dv) = q.device, q.shape, v.shape
+    dev, dtype, (T, Hk, dk), (_, Hv, dv) = q.device, q.dtype, q.shape, v.shape
     if starts is not None and (starts.dim() != 1 or starts.numel() < 1):
         raise ValueError("delta_rule: starts must be (sequences + 1) int32")
     n = starts.numel() - 1 if starts is not None else 1 if slots is None else slots.numel()
@@ -56,21 +56,25 @@ def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
         raise ValueError("delta_rule: without starts the tokens must divide into the sequences")
     if state.dim() != 4:
         raise ValueError("delta_rule: state must be (slots, heads_v, dk, dv)")
-    require(state, "delta_rule: state", torch.float32, (state.shape[0], Hv, dk, dv), dev)
-    for t, what, size in ((starts, "starts", n + 1), (slots, "slots", n), (dst, "dst", n)):
-        if t is not None:
-            require(t, f"delta_rule: {what}", torch.int32, (size,), dev)
+    n_slots = state.shape[0]
+    require(state, "delta_rule: state", torch.float32, (n_slots, Hv, dk, dv), dev)
+    if starts is not None:
+        require(starts, "delta_rule: starts", torch.int32, (n + 1,), dev)
+    if slots is not None:
+        require(slots, "delta_rule: slots", torch.int32, (n,), dev)
+    if dst is not None:
+        require(dst, "delta_rule: dst", torch.int32, (n,), dev)
+    qk_shape, v_shape, g_shape = (T, Hk, dk), (T, Hv, dv), (T, Hv, dk) if g.dim() == 3 else (T, Hv)
     if out is None:
-        out = v.new_empty((T, Hv, dv))
+        out = v.new_empty(v_shape)
     x = DeltaRows(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), out.data_ptr(),
-                  _rows(q, "q", q.dtype, (T, Hk, dk), dev), _rows(k, "k", q.dtype, (T, Hk, dk), dev),
-                  _rows(v, "v", q.dtype, (T, Hv, dv), dev),
-                  _rows(g, "g", torch.float32, (T, Hv, dk) if g.dim() == 3 else (T, Hv), dev),
-                  _rows(beta, "beta", torch.float32, (T, Hv), dev), _rows(out, "out", q.dtype, (T, Hv, dv), dev))
-    cfg = _config(q, v, g, scale)
+                  _rows(q, "q", dtype, qk_shape, dev), _rows(k, "k", dtype, qk_shape, dev), _rows(v, "v", dtype, v_shape, dev),
+                  _rows(g, "g", torch.float32, g_shape, dev), _rows(beta, "beta", torch.float32, (T, Hv), dev),
+                  _rows(out, "out", dtype, v_shape, dev))
+    cfg = DeltaConfig(ST_DTYPE[dtype], Hk, Hv, dk, dv, len(g_shape) - 2, dk ** -0.5 if scale is None else scale)
     require_device(q, "delta_rule")
     need = _lib.lib().exl3_delta_workspace_size(C.byref(cfg), T, n)
     ws = scratch(ws, need, dev, "delta_rule")
-    call("exl3_delta_rule", C.byref(cfg), C.byref(x), T, _ptr(starts), n, state.data_ptr(), state.shape[0],
+    call("exl3_delta_rule", C.byref(cfg), C.byref(x), T, _ptr(starts), n, state.data_ptr(), n_slots,
          _ptr(slots), _ptr(dst), _ptr(ws), 0 if ws is None else ws.numel(), stream_on(dev))
     return out
