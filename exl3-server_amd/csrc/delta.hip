@@ -448,7 +448,7 @@ struct alignas(16) Stage {
   E v[kC][kCol];
   float decay[DK];
   float beta[kC];
-  uint32_t v_bad[4];  // by preparing wave: the column blocks in which a value is infinite or NaN
+  uint32_t v_bad[4];  // by the wave that carried them: the column blocks in which a value is infinite or NaN
   int fine;
 };
 
@@ -810,13 +810,14 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
 
   if (wave >= kWaves) {
     // With two multiplying waves (on the first two SIMDs) the preparing ones share the other two,
-    // two on each, and the waves that would share with the multiplying ones end here.
+    // two on each, and the two waves that share with the multiplying ones only carry the values and
+    // the matrices; else the preparing waves do both.
+    constexpr int kCarriers = kWaves == 2 ? 128 : 256, kMats = 512 / kCarriers;
     const int helper = kWaves == 2 ? wave % 2 + wave / 4 * 2 : wave - kWaves;
-    if (kWaves == 2 && wave / 2 == 2) return;
-    // lane: channels ch .. of tokens 8 g ..
-    const int part = 64 * helper + lane, ch = part / 64 * (DK / 4) + m * N;
+    // lane: channels ch .. of tokens 8 g ..; as a carrier piece `part`
+    const int part = tid - 256, ch = helper * (DK / 4) + m * N;
     RawSlice<E, DK, kChannel> raw;
-    u32x4 mat[2];
+    u32x4 mat[kMats];
     int fine[2];
     float beta;
     // 8 values of a row; kPieces such pieces are the workgroup's columns
@@ -830,16 +831,46 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
     auto load = [&](int c) {
       const int t0 = s.first + c * kC;
       raw.load(a, t0, s.last - t0, h, hk, 8 * g, ch);
+    };
+    auto fetch = [&](int c) {
+      const int t0 = s.first + c * kC;
       const ChunkMats &in = mats[(size_t)c * a.heads_v];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        mat[i] = reinterpret_cast<const u32x4 *>(in.mat)[part + 256 * i];
+      for (int i = 0; i < kMats; ++i)
+        mat[i] = reinterpret_cast<const u32x4 *>(in.mat)[part + kCarriers * i];
       fine[0] = in.fine[0];
       fine[1] = in.fine[1];
       beta = in.beta[part % kC];
       const uint32_t t = min(part / kPieces, s.last - t0 - 1);
       const char *vb = chunk_rows<E>(a.v, a.v_token, t0, (int64_t)h * a.dv);
       if (has_v) val = *reinterpret_cast<const E8 *>(vb + (t * (uint32_t)a.v_token + v_col) * 2);
+    };
+    auto carry = [&](int c) {
+      St &st = stage[c & 1];
+#pragma unroll
+      for (int i = 0; i < kMats; ++i) {
+        const int at = part + kCarriers * i;  // of 512 pieces of 8 values: 4 matrices of 32 rows of 4
+        *reinterpret_cast<u32x4 *>(&st.mat[at / 128][at / 4 % 32][token_at(at / 4 % 32, at % 4 * 8)]) = mat[i];
+      }
+      if (part == 0) st.fine = fine[0] && fine[1];
+      if (part < kC) st.beta[part] = beta;
+      // infinities and NaN by their bits
+      const uint16_t inf = bitcast<uint16_t>(from_f32<E>(INFINITY));
+      typedef uint16_t U8 __attribute__((ext_vector_type(8)));
+      const U8 bits = bitcast<U8>(val) & (uint16_t)0x7fff;
+      uint16_t most = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = bits[i] > most ? bits[i] : most;
+      const uint64_t bad = __ballot(most >= inf);
+      uint32_t tiles = 0;
+#pragma unroll
+      for (int t = 0; t < kWaves; ++t) tiles |= bad & ((kPieces == 4 ? 0x3333333333333333ull : 0x0303030303030303ull) << (2 * t)) ? 1u << t : 0u;
+      if (lane == 0) st.v_bad[part / 64] = tiles;
+      if (part / kPieces >= s.last - (s.first + c * kC)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) val[i] = from_f32<E>(0.0f);
+      }
+      if (part < kC * kPieces) *reinterpret_cast<u32x4 *>(&st.v[part / kPieces][part % kPieces * 8]) = bitcast<u32x4>(val);
     };
     auto prepare = [&](int c) {
       St &st = stage[c & 1];
@@ -888,43 +919,28 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
           put_split<4>(&st.pe[0][ch + j][at], &st.pe[1][ch + j][at], k4, x4);
         }
       if (g == 0) put<N>(&st.decay[ch], all);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int at = part + 256 * i;  // of 512 pieces of 8 values: 4 matrices of 32 rows of 4
-        *reinterpret_cast<u32x4 *>(&st.mat[at / 128][at / 4 % 32][token_at(at / 4 % 32, at % 4 * 8)]) = mat[i];
-      }
-      if (part == 0) st.fine = fine[0] && fine[1];
-      if (part < kC) st.beta[part] = beta;
-      // infinities and NaN by their bits
-      const uint16_t inf = bitcast<uint16_t>(from_f32<E>(INFINITY));
-      typedef uint16_t U8 __attribute__((ext_vector_type(8)));
-      const U8 bits = bitcast<U8>(val) & (uint16_t)0x7fff;
-      uint16_t most = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) most = bits[i] > most ? bits[i] : most;
-      const uint64_t bad = __ballot(most >= inf);
-      uint32_t tiles = 0;
-#pragma unroll
-      for (int t = 0; t < kWaves; ++t) tiles |= bad & ((kPieces == 4 ? 0x3333333333333333ull : 0x0303030303030303ull) << (2 * t)) ? 1u << t : 0u;
-      if (lane == 0) st.v_bad[helper] = tiles;
-      if (part / kPieces >= s.last - (s.first + c * kC)) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) val[i] = from_f32<E>(0.0f);
-      }
-      if (part < kC * kPieces) *reinterpret_cast<u32x4 *>(&st.v[part / kPieces][part % kPieces * 8]) = bitcast<u32x4>(val);
     };
-    if (chunks > 0) {
-      load(0);
-      prepare(0);
-      if (chunks > 1) load(1);
-    }
-    lds_barrier();
-    for (int c = 0; c < chunks; ++c) {
-      if (c + 1 < chunks) {
-        prepare(c + 1);
-        if (c + 2 < chunks) load(c + 2);
+    // get(c): a chunk's rows on their way; set(c): into LDS
+    auto run = [&](auto get, auto set) {
+      if (chunks > 0) {
+        get(0);
+        set(0);
+        if (chunks > 1) get(1);
       }
       lds_barrier();
+      for (int c = 0; c < chunks; ++c) {
+        if (c + 1 < chunks) {
+          set(c + 1);
+          if (c + 2 < chunks) get(c + 2);
+        }
+        lds_barrier();
+      }
+    };
+    if constexpr (kWaves == 2) {
+      if (uniform(wave) / 2 == 2) run(fetch, carry);
+      else run(load, prepare);
+    } else {
+      run([&](int c) { load(c), fetch(c); }, [&](int c) { prepare(c), carry(c); });
     }
     return;
   }
@@ -947,7 +963,8 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
   // Whether chunk c may be multiplied.
   auto fine_chunk = [&](int c) {
     const St &st = stage[c & 1];
-    const uint32_t bad = st.v_bad[0] | st.v_bad[1] | st.v_bad[2] | st.v_bad[3];
+    uint32_t bad = st.v_bad[0] | st.v_bad[1];
+    if constexpr (kWaves != 2) bad |= st.v_bad[2] | st.v_bad[3];
     return uniform(st.fine && !(bad >> wave & 1)) != 0;
   };
   // Chunk c token by token in f32, where something in it is infinite, NaN or out of range, so
