@@ -776,13 +776,14 @@ __global__ __launch_bounds__(256, 4) void k_delta_chunk(DeltaArgs a) {
 // which all waves share, pass through LDS. The four waves behind them prepare the next chunk's
 // there (and its values), in the other of two buffers, and load the one after it: the
 // multiplying waves wait for no load, and their stores are never waited for.
-// A sequence's chunks depend on each other, so this is bound by the time of one: about 4200
-// cycles, of which 84 matrix instructions are 1350 and the splitting of the state, V and U
-// beside them most of the rest; the preparing waves need as long for some 370 vector
-// instructions each. 2048 tokens of 64 heads: 64 chunks, 144-157 us from run to run.
+// A sequence's chunks depend on each other, so this is bound by the time of one: about 4000
+// cycles of a multiplying wave, of which 84 matrix instructions are 1350 and the splitting of the
+// state, V and U beside them most of the rest, and about as long in the preparing waves. 2048 tokens of 64 heads: 64 chunks, 138-143 us from run to run.
 // (With f32 matrix instructions and no preparing waves 749 us; with f16 pairs 371; with loads
 // ahead and barriers that wait for LDS alone 193; with the preparing waves on SIMDs of their own
-// 154; with LDS pieces turned, not rows padded, and buffer loads 143.)
+// 154; with LDS pieces turned, not rows padded, and buffer loads 143; with the values and matrices
+// carried by two more waves 138, the whole call 201 -> 186.) The outputs stored 4 bytes at once, by
+// an exchange between neighbours, gained nothing.
 template <typename E, int DK, bool kChannel, int kWaves>
 __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs a, int parts) {
   constexpr int N = DK / 64, KT = DK / 16;
