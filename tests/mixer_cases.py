@@ -141,6 +141,8 @@ def choose64(x, u, temp, k, p, min_p):
     s = x[order]
     with np.errstate(invalid="ignore", over="ignore"):
         t = np.where(s == s[0], 0.0, (s[0] - s) / np.float64(temp))
+        if s[0] == np.inf:  # those of +inf share the row, at an infinite temperature too (inf / inf above)
+            t[s != s[0]] = np.inf
     w = np.exp(-t)
     w[w < 2.0 ** -45] = 0.0
     keep = len(w)

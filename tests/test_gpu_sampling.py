@@ -173,3 +173,16 @@ def test_rows_inside_each_other_are_refused(dev):
     # a single row's stride says nothing
     (a, b), (c, d) = sample_tokens(x.as_strided((1, 4000), (7, 1)), u[:1]), sample_tokens(x[:, :4000].contiguous(), u[:1])
     assert torch.equal(a, c) and torch.equal(b, d)
+
+
+@pytest.mark.parametrize("temp", [1e-45, 1e-30, 1e-3, 1e30, math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_extreme_temperatures(dev, temp, dtype):
+    # from the largest logit alone to even shares of all that are not masked; NaN as 0
+    g = gen(31, dev)
+    x, u = normal(g, (4, 3001), dtype, 3.0), uniform(g, 4)
+    x[1, 7], x[1, 2000] = math.inf, math.inf
+    x[2, :1500] = -math.inf
+    x[3, 11] = math.nan
+    check(x, u, temp, 0, 1.0, 0.0)
+    check(x, u, temp, 50, 0.9, 0.01)
